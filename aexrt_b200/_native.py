@@ -52,6 +52,15 @@ class AexrtYoloDetection(ctypes.Structure):
     _fields_ = [(name, c_float) for name in ("x1", "y1", "x2", "y2", "score", "class_id")]
 
 
+class AexrtB200AttentionDesc(ctypes.Structure):
+    _fields_ = [(name, c_uint32) for name in ("struct_size", "dtype", "num_seqs", "q_tokens", "max_q", "q_heads",
+                                              "kv_heads", "head_dim", "causal")] + [("scale", c_float)] + [
+        (name, c_uint32) for name in ("kv_tokens", "page_size", "table_columns", "table_stride")] + [
+        (name, c_uint64) for name in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride",
+                                      "k_token_stride", "k_head_stride", "k_page_stride", "v_token_stride",
+                                      "v_head_stride", "v_page_stride")]
+
+
 class AexrtError(RuntimeError):
     """A C-ABI call returned failure; the message is the library's last error."""
 
@@ -108,6 +117,14 @@ _SIGNATURES = {
                                                                                         c_void_p]),
     "aexrt_b200_act_status": (c_int, [POINTER(c_uint32)]),
     "aexrt_b200_zero": (c_int, [c_void_p, c_uint64, c_void_p]),
+    "aexrt_b200_attention_packed": (c_int, [POINTER(AexrtB200AttentionDesc)] + [c_void_p] * 8),
+    "aexrt_b200_attention_paged": (c_int, [POINTER(AexrtB200AttentionDesc)] + [c_void_p] * 9 + [c_uint64, c_void_p]),
+    "aexrt_b200_attention_paged_workspace": (c_uint64, [POINTER(AexrtB200AttentionDesc)]),
+    "aexrt_b200_attention_status": (c_int, [POINTER(c_uint32)]),
+    "aexrt_b200_page_tables": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_uint32, c_void_p,
+                                       c_uint32] + [c_void_p] * 5 + [c_uint32, c_void_p]),
+    "aexrt_b200_kv_append": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_uint32] + [c_uint64] * 4 + [c_void_p] * 3
+                             + [c_uint32, c_uint32] + [c_uint64] * 6 + [c_void_p]),
     "aexrt_b200_act_quantize_f16_noalloc": (c_int, [c_void_p] + [c_uint32] * 9 + [c_void_p, c_void_p, c_void_p]),
 }
 

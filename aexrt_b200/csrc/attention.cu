@@ -1,0 +1,296 @@
+// C ABI of attention over token sequences, its paged cache and tables (include/aexrt_b200.h):
+// checks of the description, launch shapes and the launches.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+#include "../../include/aexrt_b200.h"
+#include "attention_simple.cuh"
+#include "kv_cache.cuh"
+#include "launch.cuh"
+
+namespace aexrt {
+void set_last_error(const char* msg);
+}
+
+using namespace aexrt;
+
+namespace {
+
+int fail(const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  std::vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  set_last_error(buf);
+  return 0;
+}
+
+bool cuda_ok(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return true;
+  fail("%s: %s", what, cudaGetErrorString(e));
+  return false;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+static __device__ uint32_t g_attention_status;
+
+// This device's status word, its address resolved once per device.
+uint32_t* status_word() {
+  static std::mutex mu;
+  static uint32_t* word[128] = {};
+  int dev = 0;
+  if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return nullptr;
+  if (dev < 0 || dev >= 128) {
+    fail("device index %d out of range", dev);
+    return nullptr;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  if (!word[dev]) {
+    void* ptr = nullptr;
+    if (!cuda_ok(cudaGetSymbolAddress(&ptr, g_attention_status), "cudaGetSymbolAddress")) return nullptr;
+    word[dev] = static_cast<uint32_t*>(ptr);
+  }
+  return word[dev];
+}
+
+int log2_exact(uint32_t x) {
+  int s = 0;
+  while ((1u << s) < x) ++s;
+  return s;
+}
+
+constexpr uint64_t kMaxStride = 1ull << 38;  // elements: byte strides stay below the tensor maps' 2^40
+
+bool strides_ok(const char* what, uint64_t a, uint64_t b, uint64_t c = 0) {
+  if ((a | b | c) % 8) return fail("%s: strides must be multiples of 8 elements", what) != 0;
+  if (a >= kMaxStride || b >= kMaxStride || c >= kMaxStride) return fail("%s: stride out of range", what) != 0;
+  return true;
+}
+
+// The checks that packed and paged attention share (no pointers).
+bool desc_ok(const AexrtB200AttentionDesc* d, bool paged) {
+  const char* what = paged ? "attention_paged" : "attention_packed";
+  if (!d) return fail("%s: null description", what) != 0;
+  if (d->struct_size != sizeof(AexrtB200AttentionDesc)) return fail("%s: bad struct_size", what) != 0;
+  if (d->dtype > AEXRT_B200_DTYPE_BF16) return fail("%s: unknown dtype %u", what, d->dtype) != 0;
+  if (d->num_seqs > 65535u) return fail("%s: at most 65535 sequences", what) != 0;
+  if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8)
+    return fail("%s: head_dim must be a multiple of 8 from 8 to 128", what) != 0;
+  if (d->q_heads == 0 || d->kv_heads == 0 || d->q_heads > 65535u || d->q_heads % d->kv_heads)
+    return fail("%s: q_heads must be a multiple of kv_heads, from 1 to 65535", what) != 0;
+  if (d->q_heads / d->kv_heads > 128) return fail("%s: at most 128 query heads per kv head", what) != 0;
+  if (!(d->scale >= 0.f) || !std::isfinite(d->scale)) return fail("%s: scale must be finite and >= 0", what) != 0;
+  if (d->q_tokens > (1u << 30) || d->kv_tokens > (1u << 30)) return fail("%s: at most 2^30 rows or pages", what) != 0;
+  // rows x heads index the launch grids
+  if (static_cast<uint64_t>(d->q_tokens) * d->q_heads > (1ull << 32))
+    return fail("%s: at most 2^32 query rows times heads", what) != 0;
+  if (!strides_ok(what, d->q_token_stride, d->q_head_stride) || !strides_ok(what, d->out_token_stride, d->out_head_stride) ||
+      !strides_ok(what, d->k_token_stride, d->k_head_stride, paged ? d->k_page_stride : 0) ||
+      !strides_ok(what, d->v_token_stride, d->v_head_stride, paged ? d->v_page_stride : 0))
+    return false;
+  // rows of out that overlap would be written by several threads in no order
+  const bool tokens_inside = d->out_token_stride < d->out_head_stride;
+  const uint64_t lo = tokens_inside ? d->out_token_stride : d->out_head_stride;
+  const uint64_t hi = tokens_inside ? d->out_head_stride : d->out_token_stride;
+  const uint64_t lo_n = tokens_inside ? d->q_tokens : d->q_heads, hi_n = tokens_inside ? d->q_heads : d->q_tokens;
+  if ((lo_n > 1 && lo < d->head_dim) || (hi_n > 1 && lo_n > 0 && hi < (lo_n > 1 ? lo * (lo_n - 1) : 0) + d->head_dim))
+    return fail("%s: rows of out overlap", what) != 0;
+  if (paged) {
+    if (d->page_size < 8 || d->page_size > 1024 || (d->page_size & (d->page_size - 1)))
+      return fail("%s: page_size must be a power of two from 8 to 1024", what) != 0;
+    if (d->table_columns > (1u << 30) || d->table_stride < d->table_columns)
+      return fail("%s: table_stride below table_columns", what) != 0;
+  }
+  return true;
+}
+
+AttnParams make_params(const AexrtB200AttentionDesc* d, const void* q, const void* k, const void* v, void* out,
+                       float* lse, const int32_t* cu_q) {
+  AttnParams p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.lse = lse;
+  p.cu_q = cu_q;
+  p.q_ts = static_cast<int64_t>(d->q_token_stride);
+  p.q_hs = static_cast<int64_t>(d->q_head_stride);
+  p.o_ts = static_cast<int64_t>(d->out_token_stride);
+  p.o_hs = static_cast<int64_t>(d->out_head_stride);
+  p.k_ts = static_cast<int64_t>(d->k_token_stride);
+  p.k_hs = static_cast<int64_t>(d->k_head_stride);
+  p.k_ps = static_cast<int64_t>(d->k_page_stride);
+  p.v_ts = static_cast<int64_t>(d->v_token_stride);
+  p.v_hs = static_cast<int64_t>(d->v_head_stride);
+  p.v_ps = static_cast<int64_t>(d->v_page_stride);
+  p.num_seqs = static_cast<int>(d->num_seqs);
+  p.q_tokens = static_cast<int>(d->q_tokens);
+  p.max_q = static_cast<int>(std::min(d->max_q, 1u << 30));
+  p.q_heads = static_cast<int>(d->q_heads);
+  p.kv_heads = static_cast<int>(d->kv_heads);
+  p.group = static_cast<int>(d->q_heads / d->kv_heads);
+  p.head_dim = static_cast<int>(d->head_dim);
+  p.kv_tokens = static_cast<int>(d->kv_tokens);
+  p.causal = d->causal ? 1 : 0;
+  p.scale = d->scale;
+  return p;
+}
+
+template <typename T, bool kPaged>
+int launch_rows(const AttnParams& p, cudaStream_t st) {
+  const int64_t rows = static_cast<int64_t>(p.q_tokens) * p.q_heads;
+  launch_kernel(attention_row_kernel<T, kPaged>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, st, p);
+  return cuda_ok(cudaGetLastError(), "attention launch") ? 1 : 0;
+}
+
+}  // namespace
+
+int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, const void* k, const void* v,
+                                const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* stream) {
+  if (!desc_ok(d, false)) return 0;
+  if (d->q_tokens == 0 || d->num_seqs == 0) return 1;
+  if (!q || !cu_q || !cu_k || !out || (d->kv_tokens && (!k || !v))) return fail("attention_packed: null pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail("attention_packed: q, k, v and out must be 16-byte aligned");
+  AttnParams p = make_params(d, q, k, v, out, lse, cu_q);
+  p.cu_k = cu_k;
+  p.status = status_word();
+  if (!p.status) return 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return d->dtype == AEXRT_B200_DTYPE_F16 ? launch_rows<__half, false>(p, st) : launch_rows<__nv_bfloat16, false>(p, st);
+}
+
+uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* d) {
+  if (!desc_ok(d, true)) return ~0ull;
+  return 0;
+}
+
+int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, const void* k_cache, const void* v_cache,
+                               const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_lens, void* out,
+                               float* lse, void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (!desc_ok(d, true)) return 0;
+  if (d->q_tokens == 0 || d->num_seqs == 0 || d->max_q == 0) return 1;
+  if (!q || !cu_q || !kv_lens || !out || (d->kv_tokens && (!k_cache || !v_cache)) || (d->table_columns && !block_table))
+    return fail("attention_paged: null pointer");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return fail("attention_paged: q, caches and out must be 16-byte aligned");
+  const uint64_t need = aexrt_b200_attention_paged_workspace(d);
+  if (workspace_bytes < need || (need && (!workspace || !aligned16(workspace))))
+    return fail("attention_paged: needs %llu bytes of 16-byte aligned workspace", static_cast<unsigned long long>(need));
+  AttnParams p = make_params(d, q, k_cache, v_cache, out, lse, cu_q);
+  p.kv_lens = kv_lens;
+  p.block_table = block_table;
+  p.table_columns = static_cast<int>(d->table_columns);
+  p.table_stride = d->table_stride;
+  p.page_shift = log2_exact(d->page_size);
+  p.status = status_word();
+  if (!p.status) return 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return d->dtype == AEXRT_B200_DTYPE_F16 ? launch_rows<__half, true>(p, st) : launch_rows<__nv_bfloat16, true>(p, st);
+}
+
+int aexrt_b200_attention_status(uint32_t* status) {
+  if (!status) return fail("attention_status: null pointer");
+  uint32_t* word = status_word();
+  if (!word) return 0;
+  if (!cuda_ok(cudaMemcpy(status, word, sizeof(uint32_t), cudaMemcpyDeviceToHost), "read status")) return 0;
+  return cuda_ok(cudaMemset(word, 0, sizeof(uint32_t)), "clear status") ? 1 : 0;
+}
+
+int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uint32_t num_seqs, uint32_t page_size,
+                           int32_t* block_table, uint32_t table_columns, uint32_t table_stride,
+                           const int32_t* free_pages, uint32_t free_capacity, const int32_t* free_state_in,
+                           int32_t* free_state_out, int32_t* cu_q, int32_t* kv_lens, int32_t* slot_map,
+                           uint32_t slot_capacity, void* stream) {
+  if (num_seqs > static_cast<uint32_t>(kTablesMaxSeqs)) return fail("page_tables: at most %d requests", kTablesMaxSeqs);
+  if (page_size == 0 || page_size > 1024 || (page_size & (page_size - 1)))
+    return fail("page_tables: page_size must be a power of two up to 1024");
+  if (table_columns > (1u << 30) || table_stride < table_columns) return fail("page_tables: table_stride below table_columns");
+  if (free_capacity > (1u << 30) || slot_capacity > (1u << 30)) return fail("page_tables: at most 2^30 free pages or slots");
+  if (!free_state_in || !free_state_out || !cu_q || (num_seqs && (!ctx_lens || !new_lens || !kv_lens)) ||
+      (num_seqs && table_columns && !block_table) || (free_capacity && !free_pages) || (slot_capacity && !slot_map))
+    return fail("page_tables: null pointer");
+  TablesParams p = {};
+  p.ctx = ctx_lens;
+  p.add = new_lens;
+  p.free_pages = free_pages;
+  p.state_in = free_state_in;
+  p.table = block_table;
+  p.state_out = free_state_out;
+  p.cu_q = cu_q;
+  p.kv_lens = kv_lens;
+  p.slots = slot_map;
+  p.num_seqs = static_cast<int>(num_seqs);
+  p.page_shift = log2_exact(page_size);
+  p.columns = static_cast<int>(table_columns);
+  p.table_stride = table_stride;
+  p.free_capacity = static_cast<int>(free_capacity);
+  p.slot_capacity = static_cast<int>(slot_capacity);
+  const size_t smem = (3ull * num_seqs + 2) * sizeof(int32_t);
+  if (!cuda_ok(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (3 * kTablesMaxSeqs + 2) * static_cast<int>(sizeof(int32_t))),
+               "cudaFuncSetAttribute"))
+    return 0;
+  const unsigned ctas = std::min<unsigned>(kTablesMaxCtas, std::max<unsigned>(1, (slot_capacity + 1023) / 1024));
+  return cuda_ok(launch_kernel_cluster(page_tables_kernel, dim3(ctas), dim3(kTablesThreads), smem,
+                                       static_cast<cudaStream_t>(stream), ctas, p),
+                 "page_tables launch")
+             ? 1
+             : 0;
+}
+
+int aexrt_b200_kv_append(const void* k, const void* v, uint32_t tokens, uint32_t kv_heads, uint32_t head_dim,
+                         uint64_t k_token_stride, uint64_t k_head_stride, uint64_t v_token_stride,
+                         uint64_t v_head_stride, const int32_t* slot_map, void* k_cache, void* v_cache,
+                         uint32_t num_pages, uint32_t page_size, uint64_t k_cache_page_stride,
+                         uint64_t k_cache_token_stride, uint64_t k_cache_head_stride, uint64_t v_cache_page_stride,
+                         uint64_t v_cache_token_stride, uint64_t v_cache_head_stride, void* stream) {
+  if (head_dim == 0 || head_dim % 8 || head_dim > 65536) return fail("kv_append: head_dim must be a multiple of 8");
+  if (kv_heads == 0 || kv_heads > 65535u) return fail("kv_append: kv_heads must be from 1 to 65535");
+  if (tokens > (1u << 30)) return fail("kv_append: at most 2^30 tokens");
+  if (page_size == 0 || page_size > 1024 || (page_size & (page_size - 1)))
+    return fail("kv_append: page_size must be a power of two up to 1024");
+  if (static_cast<uint64_t>(num_pages) * page_size >= (1ull << 31)) return fail("kv_append: the cache has 2^31 slots or more");
+  if (!strides_ok("kv_append", k_token_stride, k_head_stride) || !strides_ok("kv_append", v_token_stride, v_head_stride) ||
+      !strides_ok("kv_append", k_cache_page_stride, k_cache_token_stride, k_cache_head_stride) ||
+      !strides_ok("kv_append", v_cache_page_stride, v_cache_token_stride, v_cache_head_stride))
+    return 0;
+  if (tokens == 0 || num_pages == 0) return 1;
+  if (!k || !v || !slot_map || !k_cache || !v_cache) return fail("kv_append: null pointer");
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache))
+    return fail("kv_append: k, v and the caches must be 16-byte aligned");
+  AppendParams p = {};
+  p.k = static_cast<const uint4*>(k);
+  p.v = static_cast<const uint4*>(v);
+  p.k_cache = static_cast<uint4*>(k_cache);
+  p.v_cache = static_cast<uint4*>(v_cache);
+  p.slots = slot_map;
+  p.tokens = static_cast<int>(tokens);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.row_vecs = static_cast<int>(head_dim / 8);
+  p.page_shift = log2_exact(page_size);
+  p.num_slots = static_cast<int>(num_pages * page_size);
+  p.k_ts = static_cast<int64_t>(k_token_stride / 8);
+  p.k_hs = static_cast<int64_t>(k_head_stride / 8);
+  p.v_ts = static_cast<int64_t>(v_token_stride / 8);
+  p.v_hs = static_cast<int64_t>(v_head_stride / 8);
+  p.kc_ps = static_cast<int64_t>(k_cache_page_stride / 8);
+  p.kc_ts = static_cast<int64_t>(k_cache_token_stride / 8);
+  p.kc_hs = static_cast<int64_t>(k_cache_head_stride / 8);
+  p.vc_ps = static_cast<int64_t>(v_cache_page_stride / 8);
+  p.vc_ts = static_cast<int64_t>(v_cache_token_stride / 8);
+  p.vc_hs = static_cast<int64_t>(v_cache_head_stride / 8);
+  const uint64_t pieces = static_cast<uint64_t>(tokens) * kv_heads * p.row_vecs;
+  if (pieces > (1ull << 38)) return fail("kv_append: too many elements");
+  launch_kernel(kv_append_kernel, dim3(static_cast<unsigned>((pieces + 255) / 256)), dim3(256), 0,
+                static_cast<cudaStream_t>(stream), p);
+  return cuda_ok(cudaGetLastError(), "kv_append launch") ? 1 : 0;
+}

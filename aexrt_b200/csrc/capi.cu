@@ -114,6 +114,11 @@ void pick_tile(int oh, int ow, int max_tw, int& tw, int& th) {
 namespace aexrt {
 // The library's one thread-local error message, shared by the runtime translation units.
 void set_last_error(const char* msg) { g_last_error = msg; }
+// Tensor-map encoding for the other translation units (fails with the message set).
+bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+                       const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  return encode_map(map, dt, rank, base, dims, strides_bytes, box, swizzle);
+}
 // Launch flags of this thread (aexrt_b200_set_launch_flags), read by launch_kernel (launch.cuh).
 thread_local uint32_t g_launch_flags = 0;
 uint32_t launch_flags() { return g_launch_flags; }

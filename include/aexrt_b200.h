@@ -444,6 +444,107 @@ int aexrt_b200_act_quantize_f16_noalloc(const void* x, uint32_t n, uint32_t c, u
                                         uint32_t ldc, uint32_t coff, uint32_t mode, uint32_t consumer_stride,
                                         void* q_out, float* scale_rec, void* stream);
 
+/* ---------------------------------------------------------------- attention over token sequences
+ * Softmax attention of whole prompts and of new tokens over a paged key/value cache, with the
+ * cache's tables and writes: what a step that serves sequences needs beside the fixed-map
+ * attention above (aexrt_b200_psa_attention_f16).  No counterpart in the reference, which lowers
+ * attention to MATMUL / SOFTMAX commands over fixed shapes (runtime.cpp:17305-17307).
+ *
+ *   S_ij = scale * <q_i, k_j>      o_i = sum_j exp(S_ij - lse_i) v_j      lse_i = ln sum_j exp(S_ij)
+ *
+ * over the keys j that row i sees: j < len_k and, when causal, j <= i + len_k - len_q (the last
+ * query token sees every key).  A row that sees no key gives o = 0 and lse = -inf.  Query head h
+ * reads key/value head h / (q_heads / kv_heads).  Statistics and accumulators are fp32; the
+ * probabilities are rounded to the tensors' type for the second product.
+ *
+ *   - Lengths live on the device, so a captured graph replays with other lengths.  Offsets and
+ *     lengths are cut to the tensors' extents: nothing outside them is read or written.  Rows of
+ *     q behind the last sequence are not read, and their rows of out and lse are left as they were.
+ *   - Nothing that a row does not see reaches its output, NaN and infinities in masked places,
+ *     in unused cache rows and in neighbouring sequences included.
+ *   - head_dim: a multiple of 8 from 8 to 128; q_heads / kv_heads: at most 128.  Pointers 16-byte
+ *     aligned, strides (elements) multiples of 8, each head's head_dim elements contiguous.
+ *     Every offset is computed in 64 bits.
+ *   - Launches are asynchronous on `stream` and allocate nothing. */
+#define AEXRT_B200_DTYPE_F16 0u
+#define AEXRT_B200_DTYPE_BF16 1u
+
+typedef struct AexrtB200AttentionDesc {
+    uint32_t struct_size; /* sizeof(AexrtB200AttentionDesc) */
+    uint32_t dtype;       /* AEXRT_B200_DTYPE_*: q, k, v, out */
+    uint32_t num_seqs;    /* at most 65535 */
+    uint32_t q_tokens;    /* rows of q, out and lse */
+    uint32_t max_q;       /* paged only: the most query tokens of one sequence; later ones are left out */
+    uint32_t q_heads, kv_heads, head_dim;
+    uint32_t causal;
+    float scale;          /* finite, >= 0 */
+    uint32_t kv_tokens;   /* packed: rows of k and v.  paged: pages of the cache */
+    uint32_t page_size;   /* paged: tokens per page, a power of two from 8 to 1024 */
+    uint32_t table_columns, table_stride; /* paged: columns of block_table, elements between its rows */
+    uint64_t q_token_stride, q_head_stride;
+    uint64_t out_token_stride, out_head_stride;
+    uint64_t k_token_stride, k_head_stride, k_page_stride; /* page strides: paged only */
+    uint64_t v_token_stride, v_head_stride, v_page_stride;
+} AexrtB200AttentionDesc;
+
+/* Attention over packed sequences: sequence s has query rows cu_q[s] .. cu_q[s + 1] and keys
+ * cu_k[s] .. cu_k[s + 1] (device int32 [num_seqs + 1], not decreasing).  lse (fp32
+ * [q_tokens][q_heads]) may be NULL. */
+int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* desc, const void* q, const void* k, const void* v,
+                                const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* stream);
+
+/* Attention of each sequence's new tokens (query rows cu_q[s] .. cu_q[s + 1], one or many) over its
+ * cached keys, the new tokens' own among them: key j of sequence s is row j % page_size of page
+ * block_table[s][j / page_size], j < kv_lens[s].  A table entry outside the cache reads as rows of
+ * zeros and sets AEXRT_B200_ATTENTION_BAD_PAGE.  workspace: 16-byte aligned device memory of at
+ * least aexrt_b200_attention_paged_workspace(desc) bytes (0 bytes: may be NULL), its content free before and after;
+ * calls that can overlap on the GPU each need their own. */
+int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* desc, const void* q, const void* k_cache,
+                               const void* v_cache, const int32_t* block_table, const int32_t* cu_q,
+                               const int32_t* kv_lens, void* out, float* lse, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
+/* Workspace bytes of the call on the current device; ~0 for a description that the call refuses. */
+uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* desc);
+
+/* Status of this device's attention kernels since the last read: reads and clears it
+ * (synchronises).  BAD_PAGE: a block table entry outside the cache was met.  TIMEOUT: a wait inside
+ * a kernel gave up, and outputs of that call are incomplete. */
+#define AEXRT_B200_ATTENTION_BAD_PAGE 1u
+#define AEXRT_B200_ATTENTION_TIMEOUT 2u
+int aexrt_b200_attention_status(uint32_t* status);
+
+/* The tables of a serving step, from request lengths, in one launch.  Request s holds ctx_lens[s]
+ * cached tokens and brings new_lens[s] more (negative lengths count as 0):
+ *   cu_q[num_seqs + 1]      exclusive prefix sums of new_lens;
+ *   kv_lens[s]              ctx_lens[s] + new_lens[s];
+ *   block_table[s][c]       for the columns that the new tokens add, ids taken from the free stack:
+ *                           request by request, column by column, from free_pages[top - 1]
+ *                           downwards (top = free_state_in[0]); -1 where the stack is empty.
+ *                           Columns of pages already held are read, all others left as they were;
+ *   slot_map[t]             for new token t (request by request), page * page_size + row, or -1
+ *                           where it has no page (empty stack, row of the table full) and for
+ *                           t >= cu_q[num_seqs];
+ *   free_state_out[2]       the stack's new top, and the number of pages that were missing.
+ * kv_lens may be ctx_lens and free_state_out may be free_state_in; otherwise outputs overlap
+ * nothing.  Lengths are cut so that sums stay below 2^31.  num_seqs at most 16384;
+ * slot_capacity: entries of slot_map (later tokens get none); page_size: a power of two up to
+ * 1024; free_capacity: entries of free_pages (a larger top is cut to it). */
+int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uint32_t num_seqs, uint32_t page_size,
+                           int32_t* block_table, uint32_t table_columns, uint32_t table_stride,
+                           const int32_t* free_pages, uint32_t free_capacity, const int32_t* free_state_in,
+                           int32_t* free_state_out, int32_t* cu_q, int32_t* kv_lens, int32_t* slot_map,
+                           uint32_t slot_capacity, void* stream);
+
+/* Writes rows k[t], v[t] ([kv_heads][head_dim] of 16-bit elements) to slot slot_map[t] of the
+ * caches; slots below 0 or at and above num_pages * page_size (below 2^31) are skipped.  Two tokens
+ * with the same slot leave each 16-byte piece from one of them.  Strides as in AexrtB200AttentionDesc. */
+int aexrt_b200_kv_append(const void* k, const void* v, uint32_t tokens, uint32_t kv_heads, uint32_t head_dim,
+                         uint64_t k_token_stride, uint64_t k_head_stride, uint64_t v_token_stride,
+                         uint64_t v_head_stride, const int32_t* slot_map, void* k_cache, void* v_cache,
+                         uint32_t num_pages, uint32_t page_size, uint64_t k_cache_page_stride,
+                         uint64_t k_cache_token_stride, uint64_t k_cache_head_stride, uint64_t v_cache_page_stride,
+                         uint64_t v_cache_token_stride, uint64_t v_cache_head_stride, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
