@@ -11,11 +11,14 @@
 
 #include "../../include/aexrt_b200.h"
 #include "attention_simple.cuh"
+#include "kernels_attention.cuh"
 #include "kv_cache.cuh"
 #include "launch.cuh"
 
 namespace aexrt {
 void set_last_error(const char* msg);
+bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+                       const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle);
 }
 
 using namespace aexrt;
@@ -151,6 +154,49 @@ int launch_rows(const AttnParams& p, cudaStream_t st) {
   return cuda_ok(cudaGetLastError(), "attention launch") ? 1 : 0;
 }
 
+int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, cudaStream_t st) {
+  const CUtensorMapDataType dt =
+      d->dtype == AEXRT_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint32_t tokens = kTcTileRows / p.group;
+  CUtensorMap maps[3];
+  {
+    const uint64_t dims[4] = {d->head_dim, static_cast<uint64_t>(p.group), d->kv_heads, d->q_tokens};
+    const uint64_t strides[3] = {2 * d->q_head_stride, 2 * p.group * d->q_head_stride, 2 * d->q_token_stride};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(p.group), 1, tokens};
+    if (!encode_tensor_map(&maps[0], dt, 4, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return 0;
+  }
+  for (int i = 0; i < 2; ++i) {
+    const void* base = i ? p.v : p.k;
+    const uint64_t ts = 2 * (i ? d->v_token_stride : d->k_token_stride), hs = 2 * (i ? d->v_head_stride : d->k_head_stride);
+    const uint64_t rows = std::max(1u, d->kv_tokens);
+    if (d->kv_tokens == 0) base = p.q;  // no key is ever loaded
+    bool ok;
+    if (paged) {
+      const uint64_t dims[4] = {d->head_dim, d->kv_heads, d->page_size, rows};
+      const uint64_t strides[3] = {hs, ts, 2 * (i ? d->v_page_stride : d->k_page_stride)};
+      const uint32_t box[4] = {64, 1, std::min<uint32_t>(d->page_size, kTcTileKeys), 1};
+      ok = encode_tensor_map(&maps[1 + i], dt, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    } else {
+      const uint64_t dims[3] = {d->head_dim, d->kv_heads, rows};
+      const uint64_t strides[2] = {hs, ts};
+      const uint32_t box[3] = {64, 1, kTcTileKeys};
+      ok = encode_tensor_map(&maps[1 + i], dt, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    if (!ok) return 0;
+  }
+  const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, p.head_dim);
+  if (!cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute"))
+    return 0;
+  // every sequence ends in at most one partial pair of tiles
+  const uint64_t blocks = (static_cast<uint64_t>(d->q_tokens) / (2 * tokens) + d->num_seqs) * d->kv_heads;
+  if (blocks >= (1ull << 31)) return fail("attention: %llu blocks exceed the grid", static_cast<unsigned long long>(blocks));
+  return cuda_ok(launch_kernel(k.fn, dim3(static_cast<unsigned>(blocks)), dim3(kTcBlock), k.smem, st, maps[0], maps[1],
+                               maps[2], p),
+                 "attention launch")
+             ? 1
+             : 0;
+}
+
 }  // namespace
 
 int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, const void* k, const void* v,
@@ -165,7 +211,7 @@ int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, 
   p.status = status_word();
   if (!p.status) return 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return d->dtype == AEXRT_B200_DTYPE_F16 ? launch_rows<__half, false>(p, st) : launch_rows<__nv_bfloat16, false>(p, st);
+  return launch_tc(d, p, false, st);
 }
 
 uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* d) {
@@ -194,6 +240,7 @@ int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, c
   p.status = status_word();
   if (!p.status) return 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (static_cast<uint64_t>(p.max_q) * p.group > 64) return launch_tc(d, p, true, st);
   return d->dtype == AEXRT_B200_DTYPE_F16 ? launch_rows<__half, true>(p, st) : launch_rows<__nv_bfloat16, true>(p, st);
 }
 
