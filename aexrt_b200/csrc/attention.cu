@@ -10,7 +10,7 @@
 #include <mutex>
 
 #include "../../include/aexrt_b200.h"
-#include "attention_simple.cuh"
+#include "attention_rows.cuh"
 #include "kernels_attention.cuh"
 #include "kv_cache.cuh"
 #include "launch.cuh"
@@ -147,11 +147,59 @@ AttnParams make_params(const AexrtB200AttentionDesc* d, const void* q, const voi
   return p;
 }
 
-template <typename T, bool kPaged>
-int launch_rows(const AttnParams& p, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(p.q_tokens) * p.q_heads;
-  launch_kernel(attention_row_kernel<T, kPaged>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, st, p);
-  return cuda_ok(cudaGetLastError(), "attention launch") ? 1 : 0;
+// Query rows per sequence and kv head that the few-rows kernel takes; 0: the tensor-core kernel's.
+uint32_t few_rows(const AexrtB200AttentionDesc* d) {
+  const uint64_t rows = static_cast<uint64_t>(d->max_q) * (d->q_heads / d->kv_heads);
+  return rows <= 64 ? static_cast<uint32_t>(rows) : 0;
+}
+
+int sm_count() {
+  static int cached[128] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return 148;
+  if (!cached[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
+// Runs that the list of units is cut into: two blocks per SM, fewer when even full tables have no work for them.
+uint32_t rows_grid(const AexrtB200AttentionDesc* d) {
+  const uint64_t keys = std::min<uint64_t>(static_cast<uint64_t>(d->table_columns) * d->page_size, 1ull << 31);
+  const uint64_t units = static_cast<uint64_t>(d->num_seqs) * d->kv_heads * std::max<uint64_t>(1, (keys + kRowsKeys - 1) / kRowsKeys);
+  return static_cast<uint32_t>(std::min<uint64_t>(2 * sm_count(), (units + kRowsMinUnits - 1) / kRowsMinUnits));
+}
+
+uint64_t rows_workspace(uint64_t grid, uint64_t rows, uint64_t head_dim) {
+  return grid * (sizeof(RowsRun) + 2 * rows * (head_dim + 2) * sizeof(float)) + 16;
+}
+
+int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* workspace, cudaStream_t st) {
+  RowsParams rp = {};
+  rp.a = p;
+  rp.rows = static_cast<int>(few_rows(d));
+  const uint32_t grid = rows_grid(d);
+  rp.runs = static_cast<RowsRun*>(workspace);
+  rp.parts = reinterpret_cast<float*>(rp.runs + grid);
+  rp.stats = rp.parts + 2ull * grid * rp.rows * p.head_dim;
+  const RowsKernel k = attention_rows_for(d->dtype == AEXRT_B200_DTYPE_BF16, p.head_dim, rp.rows);
+  if (!cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute"))
+    return 0;
+  if (!cuda_ok(launch_kernel(k.fn, dim3(grid), dim3(kRowsThreads), k.smem, st, rp), "attention launch")) return 0;
+  if (grid == 1) return 1;
+  // the joining launch may start while the runs end; it waits for them before it reads anything
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid - 1);
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, k.join, rp), "attention join launch") ? 1 : 0;
 }
 
 int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, cudaStream_t st) {
@@ -216,7 +264,9 @@ int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, 
 
 uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* d) {
   if (!desc_ok(d, true)) return ~0ull;
-  return 0;
+  if (d->q_tokens == 0 || d->num_seqs == 0 || d->max_q == 0) return 0;
+  const uint32_t rows = few_rows(d);
+  return rows ? rows_workspace(2ull * sm_count(), rows, d->head_dim) : 0;
 }
 
 int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, const void* k_cache, const void* v_cache,
@@ -240,8 +290,7 @@ int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, c
   p.status = status_word();
   if (!p.status) return 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (static_cast<uint64_t>(p.max_q) * p.group > 64) return launch_tc(d, p, true, st);
-  return d->dtype == AEXRT_B200_DTYPE_F16 ? launch_rows<__half, true>(p, st) : launch_rows<__nv_bfloat16, true>(p, st);
+  return few_rows(d) ? launch_rows(d, p, workspace, st) : launch_tc(d, p, true, st);
 }
 
 int aexrt_b200_attention_status(uint32_t* status) {

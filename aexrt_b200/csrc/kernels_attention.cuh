@@ -13,6 +13,16 @@ struct TcKernel {
 };
 // The tensor-core kernel (attention_tc.cuh): 16-bit type, packed or paged keys, head size 8 .. 128.
 TcKernel attention_tc_for(bool bf16, bool paged, int head_dim);
+
+// The kernel of a few rows (attention_rows.cuh; rows = most query tokens x heads per kv head, at most
+// 64) and the launch that joins what it left in parts.
+struct RowsParams;
+using RowsKernelFn = void (*)(const RowsParams);
+struct RowsKernel {
+  RowsKernelFn fn, join;
+  int smem;
+};
+RowsKernel attention_rows_for(bool bf16, int head_dim, int rows);
 constexpr int kTcBlock = 384, kTcTileRows = 128, kTcTileKeys = 128;
 
 }  // namespace aexrt
