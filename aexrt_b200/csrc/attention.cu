@@ -147,6 +147,23 @@ AttnParams make_params(const AexrtB200AttentionDesc* d, const void* q, const voi
   return p;
 }
 
+// Tensor maps of k and v: boxes of 64 elements of one head by `keys` rows (paged: by as many of a page).
+bool kv_maps(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, uint32_t keys, CUtensorMap* maps) {
+  const CUtensorMapDataType dt =
+      d->dtype == AEXRT_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int i = 0; i < 2; ++i) {
+    const void* base = i ? p.v : p.k;
+    const uint64_t ts = 2 * (i ? d->v_token_stride : d->k_token_stride), hs = 2 * (i ? d->v_head_stride : d->k_head_stride);
+    const uint64_t rows = std::max(1u, d->kv_tokens);
+    if (d->kv_tokens == 0) base = p.q;  // no key is ever loaded
+    const uint64_t dims[4] = {d->head_dim, d->kv_heads, paged ? d->page_size : rows, rows};
+    const uint64_t strides[3] = {hs, ts, 2 * (i ? d->v_page_stride : d->k_page_stride)};
+    const uint32_t box[4] = {64, 1, paged ? std::min<uint32_t>(d->page_size, keys) : keys, 1};
+    if (!encode_tensor_map(&maps[i], dt, paged ? 4 : 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
+  }
+  return true;
+}
+
 // Query rows per sequence and kv head that the few-rows kernel takes; 0: the tensor-core kernel's.
 uint32_t few_rows(const AexrtB200AttentionDesc* d) {
   const uint64_t rows = static_cast<uint64_t>(d->max_q) * (d->q_heads / d->kv_heads);
@@ -187,7 +204,10 @@ int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* work
   const RowsKernel k = attention_rows_for(d->dtype == AEXRT_B200_DTYPE_BF16, p.head_dim, rp.rows);
   if (!cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute"))
     return 0;
-  if (!cuda_ok(launch_kernel(k.fn, dim3(grid), dim3(kRowsThreads), k.smem, st, rp), "attention launch")) return 0;
+  CUtensorMap maps[2];
+  if (!kv_maps(d, p, true, kRowsKeys, maps)) return 0;
+  if (!cuda_ok(launch_kernel(k.fn, dim3(grid), dim3(kRowsThreads), k.smem, st, maps[0], maps[1], rp), "attention launch"))
+    return 0;
   if (grid == 1) return 1;
   // the joining launch may start while the runs end; it waits for them before it reads anything
   cudaLaunchAttribute attr = {};
@@ -195,7 +215,7 @@ int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* work
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid - 1);
-  cfg.blockDim = dim3(kRowsThreads);
+  cfg.blockDim = dim3(kRowsCompute);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -213,25 +233,7 @@ int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, 
     const uint32_t box[4] = {64, static_cast<uint32_t>(p.group), 1, tokens};
     if (!encode_tensor_map(&maps[0], dt, 4, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return 0;
   }
-  for (int i = 0; i < 2; ++i) {
-    const void* base = i ? p.v : p.k;
-    const uint64_t ts = 2 * (i ? d->v_token_stride : d->k_token_stride), hs = 2 * (i ? d->v_head_stride : d->k_head_stride);
-    const uint64_t rows = std::max(1u, d->kv_tokens);
-    if (d->kv_tokens == 0) base = p.q;  // no key is ever loaded
-    bool ok;
-    if (paged) {
-      const uint64_t dims[4] = {d->head_dim, d->kv_heads, d->page_size, rows};
-      const uint64_t strides[3] = {hs, ts, 2 * (i ? d->v_page_stride : d->k_page_stride)};
-      const uint32_t box[4] = {64, 1, std::min<uint32_t>(d->page_size, kTcTileKeys), 1};
-      ok = encode_tensor_map(&maps[1 + i], dt, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    } else {
-      const uint64_t dims[3] = {d->head_dim, d->kv_heads, rows};
-      const uint64_t strides[2] = {hs, ts};
-      const uint32_t box[3] = {64, 1, kTcTileKeys};
-      ok = encode_tensor_map(&maps[1 + i], dt, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    }
-    if (!ok) return 0;
-  }
+  if (!kv_maps(d, p, paged, kTcTileKeys, maps + 1)) return 0;
   const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, p.head_dim);
   if (!cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute"))
     return 0;

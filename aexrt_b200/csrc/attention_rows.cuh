@@ -4,13 +4,15 @@
 // 64) form MT tiles of 16 for the warp-level tensor instructions; each cached K and V row is read once from
 // memory, which is what bounds the kernel.  Work is a list of units, one per sequence, head and 64 keys, cut into
 // equal runs over a fixed grid: any mix of lengths fills the GPU, with one long sequence as with
-// many short ones.  A run's loads (cp.async, a ring of stages) go on across the sequences' borders.  A (sequence,
-// head) that lies inside one run is finished there; one that is cut leaves each part's
-// unnormalised sum with its maximum and normaliser in the workspace, and a second launch joins the
-// parts in a fixed order, so results do not depend on timing.
+// many short ones.  A (sequence, head) that lies inside one run is finished there; one that is cut
+// leaves each part's unnormalised sum with its maximum and normaliser in the workspace, and a second
+// launch joins the parts in a fixed order, so results do not depend on timing.
 //
-// Four warps: MT over the row tiles, 4 / MT over the keys of a stage; each keeps its own running
-// maximum and the accumulators of its keys, joined once per (sequence, head) through shared memory.
+// Four warps compute: MT over the row tiles, 4 / MT over the keys of a stage; each keeps its own
+// running maximum and the accumulators of its keys, joined once per (sequence, head) through shared
+// memory.  A fifth warp loads, one TMA box per page, ahead across the sequences' borders: with the
+// loads and their page lookups in the computing warps (cp.async), those spent 945 instructions a unit and the
+// kernel reached 3.1 TB/s at 64 x 4096 keys.
 #pragma once
 #include <climits>
 
@@ -18,7 +20,7 @@
 
 namespace aexrt {
 
-constexpr int kRowsThreads = 128;
+constexpr int kRowsCompute = 128, kRowsThreads = kRowsCompute + 32;
 constexpr int kRowsKeys = 64;     // keys of a unit
 constexpr int kRowsMinUnits = 2;  // units of a run at least: shorter runs cost more in the joining than they save
 
@@ -28,11 +30,11 @@ constexpr int rows_stages() { return DP == 128 ? 3 : 6; }
 template <int DP>
 struct RowsSmem {
   static constexpr int kHalf = kRowsKeys * DP * 2, kStage = 2 * kHalf;  // K, V
-  static constexpr int kPitch = 36;                                     // floats of a row of the joining buffer
-  static constexpr int kJoin = rows_stages<DP>() * kStage;
-  static constexpr int kStat = kJoin + 4 * 16 * kPitch * 4;             // m, l of each warp's rows
+  static_assert(kStage == 4 * 16 * DP * 4, "a stage holds the four warps' accumulators");
+  static constexpr int kStat = rows_stages<DP>() * kStage;              // m, l of each warp's rows
   static constexpr int kFix = kStat + 4 * 16 * 2 * 4;
-  static constexpr int kBytes = kFix + 3 * 128 * 4 + 16;
+  static constexpr int kBars = kFix + 3 * 128 * 4 + 16;
+  static constexpr int kBytes = kBars + 2 * rows_stages<DP>() * 8;
 };
 
 // What a run leaves for the joining: its first unit's place.
@@ -51,30 +53,23 @@ struct RowsParams {
   int rows;         // max_q * group
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <bool kTrans>
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   if constexpr (kTrans)
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (__is_same(T, __nv_bfloat16))
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
@@ -106,19 +101,28 @@ struct RowsPlace {
 __device__ __forceinline__ int64_t run_start(int64_t units, int runs, int c) { return units * c / runs; }
 
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const RowsParams rp) {
+__global__ void __launch_bounds__(kRowsThreads, 2)
+    attention_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                          const RowsParams rp) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using L = RowsSmem<DP>;
   constexpr int kStages = rows_stages<DP>(), kKeyWarps = 4 / MT, kWarpKeys = kRowsKeys / kKeyWarps;
-  constexpr int kPieces = DP / 8;                                       // 16-byte pieces of a padded row
-  constexpr int kRowStep = kRowsThreads / kPieces, kRowLoads = kRowsKeys / kRowStep;
+  constexpr int kHalves = DP / 64, kHalfBytes = kRowsKeys * 128;  // a tile: [column half][key][128 bytes], swizzled
   const AttnParams& p = rp.a;
-  float* join = reinterpret_cast<float*>(smem + L::kJoin);
   float* stat = reinterpret_cast<float*>(smem + L::kStat);
   int* fix = reinterpret_cast<int*>(smem + L::kFix);
   int* fixed = fix + 3 * 128;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* empty = full + kStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % MT, wk = warp / MT;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 4);
+    }
+    fence_mbar_init();
+  }
   grid_dep_wait();
 
   // ---- this CTA's run
@@ -136,7 +140,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
     if (lane == 0) sums[warp] = mine;
     __syncthreads();
-    units = (sums[0] + sums[1] + sums[2] + sums[3]) * p.kv_heads;
+    units = 0;
+    for (int i = 0; i < kRowsThreads / 32; ++i) units += sums[i];
+    units *= p.kv_heads;
     runs = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (units + kRowsMinUnits - 1) / kRowsMinUnits));
     const int c = blockIdx.x;
     mine_start = c < runs ? run_start(units, runs, c) : units;
@@ -186,40 +192,36 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
   }
   const int count = static_cast<int>(run_start(units, runs, blockIdx.x + 1) - mine_start);
 
-  // ---- loads: thread = one 16-byte piece of every kRowStep-th key
-  const int piece = tid % kPieces, row0 = tid / kPieces;
-  const bool in_row = piece * 8 < p.head_dim;                       // else zeros, up to a whole step of 16
-  const bool pad = !in_row && piece < (p.head_dim + 15) / 16 * 2;
-  RowsPlace ahead = at;
-  auto load = [&](int stage) {
-    const int64_t table = static_cast<int64_t>(ahead.seq) * p.table_stride;
-    const uint32_t dst = smem_u32(smem) + stage * L::kStage;
-    if (in_row || pad) {
-#pragma unroll
-      for (int i = 0; i < kRowLoads; ++i) {
-        const int r = row0 + i * kRowStep, key = ahead.tile * kRowsKeys + r;
-        int page = -1;
-        if (key < ahead.len_k) {
-          page = __ldg(p.block_table + table + (key >> p.page_shift));
-          if (page < 0 || page >= p.kv_tokens) {
-            page = -1;
-            atomicOr(p.status, kAttnBadPage);
-          }
-        }
-        const bool there = in_row && page >= 0;
-        const int64_t in_page = key & ((1 << p.page_shift) - 1);
-        const int64_t ko = there ? page * p.k_ps + in_page * p.k_ts + ahead.head * p.k_hs + piece * 8 : 0;
-        const int64_t vo = there ? page * p.v_ps + in_page * p.v_ts + ahead.head * p.v_hs + piece * 8 : 0;
-        const uint32_t to = dst + r * (DP * 2) + ((piece ^ (r & 7)) << 4);
-        cp_async16(to, static_cast<const T*>(p.k) + ko, there);
-        cp_async16(to + L::kHalf, static_cast<const T*>(p.v) + vo, there);
+  if (warp == 4) {
+    // ---- loads: a lane has one box, a page's rows of one column half of K or V
+    const int box_rows = min(1 << p.page_shift, kRowsKeys), boxes = kRowsKeys / box_rows;
+    const int box = lane % boxes, half = (lane / boxes) % kHalves, is_v = lane / (boxes * kHalves);
+    const bool on = is_v < 2;
+    bool ok = true;
+    for (int u = 0; u < count; ++u) {
+      const int stage = u % kStages;
+      int page = p.kv_tokens;  // outside the cache: zeros
+      const int key = at.tile * kRowsKeys + box * box_rows;
+      if (on && key < at.len_k) {
+        const int id = __ldg(p.block_table + at.seq * p.table_stride + (key >> p.page_shift));
+        if (id >= 0 && id < p.kv_tokens) page = id; else atomicOr(p.status, kAttnBadPage);
       }
+      ok = __all_sync(~0u, mbar_wait_bounded(empty + stage, ((u / kStages) & 1) ^ 1, p.status, kAttnTimeout));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(full + stage, L::kStage);
+      __syncwarp();
+      if (on)
+        tma_load_4d(smem + stage * L::kStage + is_v * L::kHalf + half * kHalfBytes + box * box_rows * 128,
+                    is_v ? &v_map : &k_map, full + stage, half * 64, at.head, key & ((1 << p.page_shift) - 1), page);
+      at.advance(p);
     }
-    ahead.advance(p);
-  };
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (i < count) load(i);
-    cp_async_commit();
+    // the loads in flight land before the block ends: the last ones of each stage
+    for (int i = 0; i < kStages && !ok; ++i) {
+      mbar_wait_bounded(full + i, 0, p.status, kAttnTimeout);
+      mbar_wait_bounded(full + i, 1, p.status, kAttnTimeout);
+    }
+    grid_dep_launch();
+    return;
   }
 
   const float scale = fmaxf(p.scale, 1e-30f);  // 0 would make NaN of a masked score's -inf
@@ -230,13 +232,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
   uint32_t qf[DP / 16][4];
   float o[DP / 8][4];
   float m[2], l[2];
-  int seen[2], common = 0, rows = 0, q0 = 0;
-  bool fresh = true;
+  int seen[2], common = 0, rows = 0, q0 = 0, len_q = 0;
+  bool fresh = true, dead = false;
   int part_first = at.tile;  // first tile of the current (sequence, head) that this run takes
 
   for (int u = 0; u < count; ++u) {
     if (fresh) {  // a new (sequence, head): its rows of q into registers
-      const int len_q = q_len(p, at.seq);
+      len_q = q_len(p, at.seq);
       q0 = q_start(p, at.seq);
       rows = min(len_q, p.max_q) * p.group;
       common = keys_seen(0, len_q, at.len_k, p.causal);
@@ -245,13 +247,16 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
         const int r = wr * 16 + g + 8 * e, token = r / p.group;
         const bool on = r < rows;
         seen[e] = on ? keys_seen(token, len_q, at.len_k, p.causal) : 0;
-        const T* src = static_cast<const T*>(p.q) + (q0 + token) * p.q_ts + (at.head * p.group + r % p.group) * p.q_hs;
+        // rows and columns that are not there read the first ones and count 0: no branch between the loads
+        const int64_t from = on ? token * p.q_ts + (r % p.group) * p.q_hs : 0;
+        const T* src = static_cast<const T*>(p.q) + q0 * p.q_ts + at.head * p.group * p.q_hs + from;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
           for (int f = 0; f < 2; ++f) {
             const int d = k * 16 + f * 8 + quad * 2;
-            qf[k][e + 2 * f] = on && d < p.head_dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+            const uint32_t x = __ldg(reinterpret_cast<const uint32_t*>(src + (d < p.head_dim ? d : 0)));
+            qf[k][e + 2 * f] = on && d < p.head_dim ? x : 0u;
           }
         m[e] = -INFINITY;
         l[e] = 0.f;
@@ -263,49 +268,59 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
       part_first = at.tile;
       fresh = false;
     }
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    {
-      const int next = u + kStages - 1;
-      if (next < count) load(next % kStages);
-      cp_async_commit();
-    }
+    // after a wait that gave up, the warp goes on without waiting (the status tells): the barriers between the
+    // warps still see all of them
+    if (!dead) dead = !mbar_wait_bounded(full + u % kStages, (u / kStages) & 1, p.status, kAttnTimeout);
+    __syncwarp();
     uint8_t* stage = smem + (u % kStages) * L::kStage;
     const uint32_t ks = smem_u32(stage), vs = ks + L::kHalf;
     const int key0 = at.tile * kRowsKeys;
-    if (key0 + kRowsKeys > common && common < at.len_k) {
-      // P is 0 where a row does not see a key, but 0 * inf and 0 * NaN are not: non-finite values of
-      // keys that only some rows see are taken out here and put back into the rows that do
-      const int lo = max(0, common - key0), hi = min(kRowsKeys, at.len_k - key0);
-      for (int r = lo + row0; r < hi; r += kRowStep)
-        if (in_row) {
-          uint4* v = reinterpret_cast<uint4*>(stage + L::kHalf + r * (DP * 2) + ((piece ^ (r & 7)) << 4));
+    const int last = at.len_k - key0;
+    const bool clean = last < kRowsKeys || common - key0 < kRowsKeys;
+    if (clean) {
+      // P is 0 where a row does not see a key, but 0 * inf and 0 * NaN are not: rows behind the last key
+      // become zeros, and non-finite values of keys that only some rows see are taken out and put back
+      // into the outputs of the rows that do
+      for (int i = tid; i < kRowsKeys * 8 * kHalves; i += kRowsCompute) {
+        const int r = (i >> 3) % kRowsKeys, half = i / (kRowsKeys * 8);
+        uint4* v = reinterpret_cast<uint4*>(stage + L::kHalf + half * kHalfBytes + r * 128) + (i & 7);
+        if (r >= last) {
+          *v = make_uint4(0, 0, 0, 0);
+        } else if (r >= common - key0) {
           const uint4 x = *v;
           if (non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w)) {
-            *v = take_non_finite<T>(x, key0 + r, piece * 8, fix);
+            *v = take_non_finite<T>(x, key0 + r, half * 64 + ((i & 7) ^ (r & 7)) * 8, fix);
             *fixed = 1;
           }
         }
-      __syncthreads();
+      }
+      fence_proxy_async_smem();  // before a later TMA write of this stage
+      named_bar_sync(1, kRowsCompute);
     }
 
-    // ---- S = Q K^T for this warp's keys
+    // ---- S = Q K^T for this warp's keys, 16 at a time: all of their K first, then two sums over
+    // the even and the odd steps, so that neither the loads nor the sums wait for one another
     float s[kWarpKeys / 8][4];
 #pragma unroll
-    for (int n = 0; n < kWarpKeys / 8; ++n)
+    for (int n = 0; n < kWarpKeys / 16; ++n) {
+      const int key = wk * kWarpKeys + n * 16 + ((lane >> 4) << 3) + (lane & 7);
+      uint32_t b[DP / 16][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      for (int k = 0; k < DP / 16; ++k) {
+        const int c = 2 * k + ((lane >> 3) & 1);
+        ldmatrix4<false>(ks + (c >> 3) * kHalfBytes + key * 128 + (((c & 7) ^ (key & 7)) << 4), b[k]);
+      }
+      float t[2][2][4] = {};
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      if (k < steps) {
-#pragma unroll
-        for (int n = 0; n < kWarpKeys / 16; ++n) {
-          const int key = wk * kWarpKeys + n * 16 + ((lane >> 4) << 3) + (lane & 7), c = 2 * k + ((lane >> 3) & 1);
-          uint32_t b[4];
-          ldmatrix4<false>(ks + key * (DP * 2) + ((c ^ (key & 7)) << 4), b);
-          mma_16816<T>(s[2 * n], qf[k], b[0], b[1]);
-          mma_16816<T>(s[2 * n + 1], qf[k], b[2], b[3]);
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < steps) {
+          mma_16816<T>(t[k & 1][0], qf[k], b[k][0], b[k][1]);
+          mma_16816<T>(t[k & 1][1], qf[k], b[k][2], b[k][3]);
         }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[2 * n][e] = t[0][0][e] + t[1][0][e];
+        s[2 * n + 1][e] = t[0][1][e] + t[1][1][e];
       }
     }
     const int keyw = key0 + wk * kWarpKeys;
@@ -357,12 +372,14 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
       for (int n = 0; n < DP / 16; ++n) {
         if (n < steps) {
           uint32_t b[4];
-          ldmatrix4<true>(vs + key * (DP * 2) + (((2 * n + (lane >> 4)) ^ (key & 7)) << 4), b);
+          const int c = 2 * n + (lane >> 4);
+          ldmatrix4<true>(vs + (c >> 3) * kHalfBytes + key * 128 + (((c & 7) ^ (key & 7)) << 4), b);
           mma_16816<T>(o[2 * n], a, b[0], b[1]);
           mma_16816<T>(o[2 * n + 1], a, b[2], b[3]);
         }
       }
     }
+
 
     // ---- the end of a (sequence, head), or of the run: join the key warps, write
     if (at.tile + 1 == at.tiles || u + 1 == count) {
@@ -377,74 +394,73 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
           stat[(warp * 16 + g + 8 * e) * 2 + 1] = l[e];
         }
       }
-      __syncthreads();
+      named_bar_sync(1, kRowsCompute);  // no warp reads the stage's K and V any more: it holds the accumulators now
       const bool patch = *fixed != 0;
-      // every thread scales its accumulators to its rows' maximum over the key warps
-      float f[2];
+      // [warp][row][DP] floats, columns swizzled by the row so that a warp's stores spread over the banks
+      float* join = reinterpret_cast<float*>(stage);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float all = -INFINITY;
+        if (wr * 16 + g + 8 * e < rows) {
+          float all = -INFINITY;  // the row's maximum over the key warps
 #pragma unroll
-        for (int w = 0; w < kKeyWarps; ++w) all = fmaxf(all, stat[((w * MT + wr) * 16 + g + 8 * e) * 2]);
-        f[e] = m[e] == -INFINITY ? 0.f : exp2_sfu((m[e] - all) * sl2);
-        if (m[e] == all) f[e] = 1.f;  // infinite maxima too
-      }
-      for (int c0 = 0; c0 < p.head_dim; c0 += 32) {  // 32 columns at a time
+          for (int w = 0; w < kKeyWarps; ++w) all = fmaxf(all, stat[((w * MT + wr) * 16 + g + 8 * e) * 2]);
+          // equal maxima, infinite ones too: 1
+          const float f = m[e] == all ? 1.f : (m[e] == -INFINITY ? 0.f : exp2_sfu((m[e] - all) * sl2));
+          float* row = join + (warp * 16 + g + 8 * e) * DP;
 #pragma unroll
-        for (int n = 0; n < DP / 8; ++n)
-          if (n * 8 >= c0 && n * 8 < c0 + 32) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<float2*>(join + (warp * 16 + g + 8 * e) * L::kPitch + n * 8 - c0 + quad * 2) =
-                  make_float2(o[n][2 * e] * f[e], o[n][2 * e + 1] * f[e]);
-          }
-        __syncthreads();
-        for (int i = tid; i < rows * 4; i += kRowsThreads) {  // 8 columns of one row
-          const int r = i >> 2, c = (i & 3) * 8, t = r >> 4;
-          if (c0 + c >= p.head_dim) continue;
-          float y[8] = {}, all = -INFINITY, norm = 0.f;
-#pragma unroll
-          for (int w = 0; w < kKeyWarps; ++w) {
-            const float* src = join + ((w * MT + t) * 16 + (r & 15)) * L::kPitch + c;
-            all = fmaxf(all, stat[((w * MT + t) * 16 + (r & 15)) * 2]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] += src[e];
-          }
-#pragma unroll
-          for (int w = 0; w < kKeyWarps; ++w) {
-            const float* st = stat + ((w * MT + t) * 16 + (r & 15)) * 2;
-            norm += st[0] == all ? st[1] : (st[0] == -INFINITY ? 0.f : st[1] * exp2_sfu((st[0] - all) * sl2));
-          }
-          const int token = r / p.group, qh = at.head * p.group + r % p.group;
-          const int sees = keys_seen(token, q_len(p, at.seq), at.len_k, p.causal);
-          const float inv = !whole ? 1.f : (norm == 0.f ? 0.f : 1.f / norm);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            y[e] *= inv;
-            if (patch) y[e] = put_back(y[e], fix, c0 + c + e, sees);
-          }
-          if (whole) {
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + c0 + c) =
-                make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
-            if (c0 + c == 0 && p.lse)
-              p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
-          } else {
-            float* dst = rp.parts + (static_cast<int64_t>(slot) * rp.rows + r) * p.head_dim + c0 + c;
-            *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
-            if (c0 + c == 0)
-              *reinterpret_cast<float2*>(rp.stats + (static_cast<int64_t>(slot) * rp.rows + r) * 2) = make_float2(all, norm);
-          }
+          for (int n = 0; n < DP / 8; ++n)
+            *reinterpret_cast<float2*>(row + ((n * 8 + quad * 2) ^ (g << 3))) = make_float2(o[n][2 * e] * f, o[n][2 * e + 1] * f);
         }
-        __syncthreads();
+      }
+      named_bar_sync(1, kRowsCompute);
+      constexpr int kVecs = DP / 8;
+      for (int i = tid; i < rows * kVecs; i += kRowsCompute) {  // 8 columns of one row
+        const int r = i / kVecs, c = i % kVecs * 8;
+        if (c >= p.head_dim) continue;
+        float y[8] = {}, all = -INFINITY, norm = 0.f;
+#pragma unroll
+        for (int w = 0; w < kKeyWarps; ++w) all = fmaxf(all, stat[((w * MT + (r >> 4)) * 16 + (r & 15)) * 2]);
+#pragma unroll
+        for (int w = 0; w < kKeyWarps; ++w) {
+          const int at_row = (w * MT + (r >> 4)) * 16 + (r & 15);
+          const float2 st = *reinterpret_cast<const float2*>(stat + at_row * 2);
+          norm += st.x == all ? st.y : (st.x == -INFINITY ? 0.f : st.y * exp2_sfu((st.x - all) * sl2));
+          const float4* src = reinterpret_cast<const float4*>(join + at_row * DP + (c ^ ((r & 7) << 3)));
+          const float4 a = src[0], b = src[1];
+          y[0] += a.x, y[1] += a.y, y[2] += a.z, y[3] += a.w, y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
+        }
+        const int token = r / p.group, qh = at.head * p.group + r % p.group;
+        const float inv = !whole ? 1.f : (norm == 0.f ? 0.f : 1.f / norm);
+        const int sees = patch ? keys_seen(token, len_q, at.len_k, p.causal) : 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y[e] *= inv;
+          if (patch) y[e] = put_back(y[e], fix, c + e, sees);
+        }
+        if (whole) {
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + c) =
+              make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+          if (c == 0 && p.lse)
+            p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
+        } else {
+          const int64_t part = static_cast<int64_t>(slot) * rp.rows + r;
+          float4* dst = reinterpret_cast<float4*>(rp.parts + part * p.head_dim + c);
+          dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+          dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+          if (c == 0) *reinterpret_cast<float2*>(rp.stats + part * 2) = make_float2(all, norm);
+        }
       }
       if (patch) {
-        for (int i = tid; i < 3 * 128; i += kRowsThreads) fix[i] = INT_MAX;
+        named_bar_sync(1, kRowsCompute);
+        for (int i = tid; i < 3 * 128; i += kRowsCompute) fix[i] = INT_MAX;
         if (tid == 0) *fixed = 0;
-        __syncthreads();
       }
+      fence_proxy_async_smem();      // these accesses before the stage's next TMA write
+      named_bar_sync(1, kRowsCompute);  // and before the next statistics
       fresh = true;
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + u % kStages);
     at.advance(p);
   }
   grid_dep_launch();
@@ -453,7 +469,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attention_rows_kernel(const R
 // Joins the parts of every (sequence, head) that was cut: block c - 1 takes the one that run c goes on
 // with, when run c is the first to do so.  Parts are summed in the order of the keys.
 template <typename T>
-__global__ void __launch_bounds__(kRowsThreads) attention_rows_join_kernel(const RowsParams rp) {
+__global__ void __launch_bounds__(kRowsCompute) attention_rows_join_kernel(const RowsParams rp) {
   grid_dep_launch();
   grid_dep_wait();
   const AttnParams& p = rp.a;
@@ -466,7 +482,7 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_join_kernel(const
   while (c + parts - 1 < run.runs && run_start(run.units, run.runs, c + parts - 1) < end) ++parts;
   const float scale = fmaxf(p.scale, 1e-30f), sl2 = scale * 1.4426950408889634f;
   const int rows = min(q_len(p, run.seq), p.max_q) * p.group, q0 = q_start(p, run.seq), vecs = p.head_dim / 8;
-  for (int i = threadIdx.x; i < rows * vecs; i += kRowsThreads) {
+  for (int i = threadIdx.x; i < rows * vecs; i += kRowsCompute) {
     const int r = i / vecs, d = i % vecs * 8;
     auto row_of = [&](int k) { return (static_cast<int64_t>(2 * (c - 1 + k) + (k == 0 ? 1 : 0))) * rp.rows + r; };
     float all = -INFINITY;

@@ -17,9 +17,9 @@ TcKernel attention_tc_for(bool bf16, bool paged, int head_dim);
 // The kernel of a few rows (attention_rows.cuh; rows = most query tokens x heads per kv head, at most
 // 64) and the launch that joins what it left in parts.
 struct RowsParams;
-using RowsKernelFn = void (*)(const RowsParams);
 struct RowsKernel {
-  RowsKernelFn fn, join;
+  void (*fn)(const CUtensorMap, const CUtensorMap, const RowsParams);
+  void (*join)(const RowsParams);
   int smem;
 };
 RowsKernel attention_rows_for(bool bf16, int head_dim, int rows);
