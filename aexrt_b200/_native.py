@@ -117,9 +117,10 @@ _SIGNATURES = {
                                                                                         c_void_p]),
     "aexrt_b200_act_status": (c_int, [POINTER(c_uint32)]),
     "aexrt_b200_zero": (c_int, [c_void_p, c_uint64, c_void_p]),
-    "aexrt_b200_attention_packed": (c_int, [POINTER(AexrtB200AttentionDesc)] + [c_void_p] * 8),
-    "aexrt_b200_attention_paged": (c_int, [POINTER(AexrtB200AttentionDesc)] + [c_void_p] * 9 + [c_uint64, c_void_p]),
-    "aexrt_b200_attention_paged_workspace": (c_uint64, [POINTER(AexrtB200AttentionDesc)]),
+    # descriptions by address: a structure or its bytes
+    "aexrt_b200_attention_packed": (c_int, [c_void_p] * 9),
+    "aexrt_b200_attention_paged": (c_int, [c_void_p] * 10 + [c_uint64, c_void_p]),
+    "aexrt_b200_attention_paged_workspace": (c_uint64, [c_void_p]),
     "aexrt_b200_attention_status": (c_int, [POINTER(c_uint32)]),
     "aexrt_b200_page_tables": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_uint32, c_void_p,
                                        c_uint32] + [c_void_p] * 5 + [c_uint32, c_void_p]),

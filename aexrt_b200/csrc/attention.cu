@@ -64,6 +64,26 @@ uint32_t* status_word() {
   return word[dev];
 }
 
+// Raises a kernel's dynamic shared memory limit, once per kernel and device.
+bool raise_smem(const void* fn, int bytes) {
+  struct Raised {
+    const void* fn;
+    int dev;
+  };
+  static std::mutex mu;
+  static Raised raised[512];
+  static int count = 0;
+  int dev = 0;
+  if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return false;
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < count; ++i)
+    if (raised[i].fn == fn && raised[i].dev == dev) return true;
+  if (!cuda_ok(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute"))
+    return false;
+  if (count < 512) raised[count++] = Raised{fn, dev};
+  return true;
+}
+
 int log2_exact(uint32_t x) {
   int s = 0;
   while ((1u << s) < x) ++s;
@@ -202,8 +222,7 @@ int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* work
   rp.parts = reinterpret_cast<float*>(rp.runs + grid);
   rp.stats = rp.parts + 2ull * grid * rp.rows * p.head_dim;
   const RowsKernel k = attention_rows_for(d->dtype == AEXRT_B200_DTYPE_BF16, p.head_dim, rp.rows);
-  if (!cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute"))
-    return 0;
+  if (!raise_smem(reinterpret_cast<const void*>(k.fn), k.smem)) return 0;
   CUtensorMap maps[2];
   if (!kv_maps(d, p, true, kRowsKeys, maps)) return 0;
   if (!cuda_ok(launch_kernel(k.fn, dim3(grid), dim3(kRowsThreads), k.smem, st, maps[0], maps[1], rp), "attention launch"))
@@ -235,8 +254,7 @@ int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, 
   }
   if (!kv_maps(d, p, paged, kTcTileKeys, maps + 1)) return 0;
   const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, p.head_dim);
-  if (!cuda_ok(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute"))
-    return 0;
+  if (!raise_smem(reinterpret_cast<const void*>(k.fn), k.smem)) return 0;
   // every sequence ends in at most one partial pair of tiles
   const uint64_t blocks = (static_cast<uint64_t>(d->q_tokens) / (2 * tokens) + d->num_seqs) * d->kv_heads;
   if (blocks >= (1ull << 31)) return fail("attention: %llu blocks exceed the grid", static_cast<unsigned long long>(blocks));
@@ -333,9 +351,8 @@ int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uin
   p.free_capacity = static_cast<int>(free_capacity);
   p.slot_capacity = static_cast<int>(slot_capacity);
   const size_t smem = (3ull * num_seqs + 2) * sizeof(int32_t);
-  if (!cuda_ok(cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (3 * kTablesMaxSeqs + 2) * static_cast<int>(sizeof(int32_t))),
-               "cudaFuncSetAttribute"))
+  if (!raise_smem(reinterpret_cast<const void*>(page_tables_kernel),
+                  (3 * kTablesMaxSeqs + 2) * static_cast<int>(sizeof(int32_t))))
     return 0;
   const unsigned ctas = std::min<unsigned>(kTablesMaxCtas, std::max<unsigned>(1, (slot_capacity + 1023) / 1024));
   return cuda_ok(launch_kernel_cluster(page_tables_kernel, dim3(ctas), dim3(kTablesThreads), smem,

@@ -37,13 +37,12 @@ struct RowsSmem {
   static constexpr int kBytes = kBars + 2 * rows_stages<DP>() * 8;
 };
 
-// What a run leaves for the joining: its first unit's place.
+// What a run leaves for the joining when it is the first to go on with a (sequence, head) that the run
+// before it began: the parts it is in (this run's predecessor's, its own and its successors'; 0:
+// nothing to join), its query rows and where they lie.
 struct RowsRun {
-  int64_t start, units;  // first unit of the run, units of the whole call
-  int seq, head, tile, tiles;  // the first unit's sequence, head, tile, and the tiles of that (sequence, head)
-  int runs, pad[3];      // runs of the call
+  int parts, rows, q0, head;
 };
-static_assert(sizeof(RowsRun) == 48, "16-byte multiple");
 
 struct RowsParams {
   AttnParams a;
@@ -97,8 +96,23 @@ struct RowsPlace {
   }
 };
 
-// First unit of run c when `units` are cut into `runs`.
-__device__ __forceinline__ int64_t run_start(int64_t units, int runs, int c) { return units * c / runs; }
+// `units` cut into `runs`: the first units % runs of them are one longer.
+struct RowsCut {
+  int64_t per;
+  int runs, more;
+  __device__ __forceinline__ RowsCut(int64_t units, int grid) {
+    runs = static_cast<int>(min(static_cast<int64_t>(grid), (units + kRowsMinUnits - 1) / kRowsMinUnits));
+    if (units >> 31) {
+      per = units / max(runs, 1);
+      more = static_cast<int>(units % max(runs, 1));
+    } else {  // the usual case: a 32-bit division
+      const uint32_t n = static_cast<uint32_t>(units), r = static_cast<uint32_t>(max(runs, 1));
+      per = n / r;
+      more = static_cast<int>(n % r);
+    }
+  }
+  __device__ __forceinline__ int64_t start(int c) const { return c * per + min(c, more); }
+};
 
 template <typename T, int DP, int MT>
 __global__ void __launch_bounds__(kRowsThreads, 2)
@@ -125,72 +139,65 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   }
   grid_dep_wait();
 
-  // ---- this CTA's run
+  // ---- this CTA's run: the units of every sequence are summed, then the one that holds the first unit found
   for (int i = tid; i < 3 * 128; i += kRowsThreads) fix[i] = INT_MAX;
   if (tid == 0) *fixed = 0;
-  int64_t units, mine_start;
-  int runs;
-  RowsPlace at;
-  {
-    __shared__ int64_t sums[kRowsThreads / 32];
-    __shared__ RowsPlace found;
-    int64_t mine = 0;
-    for (int s = tid; s < p.num_seqs; s += kRowsThreads) mine += rows_tiles(p, s);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
-    if (lane == 0) sums[warp] = mine;
-    __syncthreads();
-    units = 0;
-    for (int i = 0; i < kRowsThreads / 32; ++i) units += sums[i];
-    units *= p.kv_heads;
-    runs = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (units + kRowsMinUnits - 1) / kRowsMinUnits));
-    const int c = blockIdx.x;
-    mine_start = c < runs ? run_start(units, runs, c) : units;
-    if (c < runs && warp == 0) {  // the sequence that holds unit mine_start
-      int64_t before = 0;
-      for (int base = 0; base < p.num_seqs; base += 32) {
-        const int s = base + lane;
-        const int n = s < p.num_seqs ? rows_tiles(p, s) : 0;
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int z = __shfl_up_sync(~0u, sum, o);
-          if (lane >= o) sum += z;
-        }
-        const uint32_t past = __ballot_sync(~0u, (before + sum) * p.kv_heads > mine_start);
-        if (past) {
-          const int src = __ffs(past) - 1;
-          if (lane == src) {
-            const int64_t off = mine_start - (before + sum - n) * p.kv_heads;
-            found.seq = s;
-            found.head = static_cast<int>(off / n);
-            found.tile = static_cast<int>(off % n);
-            found.tiles = n;
-            found.len_k = k_len<true>(p, s);
-          }
-          break;
-        }
-        before += __shfl_sync(~0u, sum, 31);
-      }
+  constexpr int kWarps = kRowsThreads / 32;
+  __shared__ int64_t sums[kWarps];
+  __shared__ RowsPlace found;
+  auto up_to = [&](int64_t n) {  // inclusive sum over the warp
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t z = __shfl_up_sync(~0u, n, o);
+      if (lane >= o) n += z;
     }
-    __syncthreads();
-    at = found;
-    if (tid == 0) {
-      RowsRun r = {};
-      r.start = mine_start;
-      r.units = units;
-      r.runs = runs;
-      if (c < runs) {
-        r.seq = at.seq;
-        r.head = at.head;
-        r.tile = at.tile;
-        r.tiles = at.tiles;
-      }
-      rp.runs[c] = r;
-    }
-    if (c >= runs) return;
+    return n;
+  };
+  // one sequence per thread, or one block of sequences when there are more of them than threads
+  const int each = (p.num_seqs + kRowsThreads - 1) / kRowsThreads, s0 = min(tid * each, p.num_seqs);
+  const int s1 = min(s0 + each, p.num_seqs);
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += rows_tiles(p, s);
+  const int64_t incl = up_to(mine);
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  int64_t units = 0, before = incl - mine;  // tiles, of all sequences and of those before this thread's
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += sums[i];
+    units += sums[i];
   }
-  const int count = static_cast<int>(run_start(units, runs, blockIdx.x + 1) - mine_start);
+  units *= p.kv_heads;
+  before *= p.kv_heads;
+  const RowsCut cut(units, gridDim.x);
+  const int64_t start = cut.start(blockIdx.x);
+  const int count = static_cast<int>(cut.start(blockIdx.x + 1) - start);
+  if (static_cast<int>(blockIdx.x) >= cut.runs) {
+    if (tid == 0) rp.runs[blockIdx.x].parts = 0;
+    return;
+  }
+  if (start >= before && start < before + mine * p.kv_heads) {
+    for (int s = s0; s < s1; ++s) {
+      const int n = rows_tiles(p, s);
+      const int64_t here = static_cast<int64_t>(n) * p.kv_heads;
+      if (start < before + here) {
+        const int64_t off = start - before;
+        found.seq = s;
+        if (off >> 31) {
+          found.head = static_cast<int>(off / n);
+          found.tile = static_cast<int>(off % n);
+        } else {
+          found.head = static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(n));
+          found.tile = static_cast<int>(static_cast<uint32_t>(off) % static_cast<uint32_t>(n));
+        }
+        found.tiles = n;
+        found.len_k = k_len<true>(p, s);
+        break;
+      }
+      before += here;
+    }
+  }
+  __syncthreads();
+  RowsPlace at = found;
 
   if (warp == 4) {
     // ---- loads: a lane has one box, a page's rows of one column half of K or V
@@ -198,6 +205,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     const int box = lane % boxes, half = (lane / boxes) % kHalves, is_v = lane / (boxes * kHalves);
     const bool on = is_v < 2;
     bool ok = true;
+    const RowsPlace begin = at;
     for (int u = 0; u < count; ++u) {
       const int stage = u % kStages;
       int page = p.kv_tokens;  // outside the cache: zeros
@@ -214,6 +222,20 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         tma_load_4d(smem + stage * L::kStage + is_v * L::kHalf + half * kHalfBytes + box * box_rows * 128,
                     is_v ? &v_map : &k_map, full + stage, half * 64, at.head, key & ((1 << p.page_shift) - 1), page);
       at.advance(p);
+    }
+    if (lane == 0) {
+      // is this run the first that goes on with its first (sequence, head)?  Then it heads the joining.
+      const int c = blockIdx.x;
+      const int64_t first = start - begin.tile, end = first + begin.tiles;
+      RowsRun r = {};
+      if (begin.tile > 0 && cut.start(c - 1) <= first) {
+        r.parts = 1;
+        while (c + r.parts - 1 < cut.runs && cut.start(c + r.parts - 1) < end) ++r.parts;
+        r.rows = min(q_len(p, begin.seq), p.max_q) * p.group;
+        r.q0 = q_start(p, begin.seq);
+        r.head = begin.head;
+      }
+      rp.runs[c] = r;
     }
     // the loads in flight land before the block ends: the last ones of each stage
     for (int i = 0; i < kStages && !ok; ++i) {
@@ -466,8 +488,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   grid_dep_launch();
 }
 
-// Joins the parts of every (sequence, head) that was cut: block c - 1 takes the one that run c goes on
-// with, when run c is the first to do so.  Parts are summed in the order of the keys.
+// Joins the parts of every (sequence, head) that was cut: block c - 1 takes the one that run c heads.
+// A thread has 8 columns of a row; parts are summed in the order of the keys.
 template <typename T>
 __global__ void __launch_bounds__(kRowsCompute) attention_rows_join_kernel(const RowsParams rp) {
   grid_dep_launch();
@@ -475,37 +497,50 @@ __global__ void __launch_bounds__(kRowsCompute) attention_rows_join_kernel(const
   const AttnParams& p = rp.a;
   const int c = blockIdx.x + 1;
   const RowsRun run = rp.runs[c];
-  if (c >= run.runs || run.tile == 0) return;
-  const int64_t first = run.start - run.tile, end = first + run.tiles;
-  if (run_start(run.units, run.runs, c - 1) > first) return;
-  int parts = 1;  // run c - 1's, then one for each run that starts before the end
-  while (c + parts - 1 < run.runs && run_start(run.units, run.runs, c + parts - 1) < end) ++parts;
+  if (run.parts == 0) return;
   const float scale = fmaxf(p.scale, 1e-30f), sl2 = scale * 1.4426950408889634f;
-  const int rows = min(q_len(p, run.seq), p.max_q) * p.group, q0 = q_start(p, run.seq), vecs = p.head_dim / 8;
-  for (int i = threadIdx.x; i < rows * vecs; i += kRowsCompute) {
+  const int vecs = p.head_dim / 8;
+  for (int i = threadIdx.x; i < run.rows * vecs; i += kRowsCompute) {
     const int r = i / vecs, d = i % vecs * 8;
+    // part k is run c - 1 + k's: the second slot of the first run, the first slot of the others
     auto row_of = [&](int k) { return (static_cast<int64_t>(2 * (c - 1 + k) + (k == 0 ? 1 : 0))) * rp.rows + r; };
-    float all = -INFINITY;
-    for (int k = 0; k < parts; ++k) all = fmaxf(all, rp.stats[row_of(k) * 2]);
-    float y[8] = {}, norm = 0.f;
-    for (int k = 0; k < parts; ++k) {
-      const float2 st = *reinterpret_cast<const float2*>(rp.stats + row_of(k) * 2);
-      const float f = st.x == all ? 1.f : (st.x == -INFINITY ? 0.f : exp2_sfu((st.x - all) * sl2));
-      norm = fmaf(st.y, f, norm);
-      const float4* src = reinterpret_cast<const float4*>(rp.parts + row_of(k) * p.head_dim + d);
-      const float4 a = src[0], b = src[1];
-      const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    float y[8] = {}, all = -INFINITY, norm = 0.f;
+    for (int k0 = 0; k0 < run.parts; k0 += 4) {  // four parts' loads at a time
+      float2 st[4];
+      float4 a[4], b[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = f == 0.f && !isfinite(x[e]) ? y[e] + x[e] : fmaf(x[e], f, y[e]);
+      for (int k = 0; k < 4; ++k) {
+        const int64_t row = row_of(min(k0 + k, run.parts - 1));
+        st[k] = *reinterpret_cast<const float2*>(rp.stats + row * 2);
+        const float4* src = reinterpret_cast<const float4*>(rp.parts + row * p.head_dim + d);
+        a[k] = src[0];
+        b[k] = src[1];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k0 + k >= run.parts) break;
+        if (st[k].x > all) {  // a new maximum: what is summed so far shrinks
+          const float f = all == -INFINITY ? 0.f : exp2_sfu((all - st[k].x) * sl2);
+          norm *= f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = f == 0.f && !isfinite(y[e]) ? y[e] : y[e] * f;
+          all = st[k].x;
+        }
+        const float f = st[k].x == all ? 1.f : (st[k].x == -INFINITY ? 0.f : exp2_sfu((st[k].x - all) * sl2));
+        norm = fmaf(st[k].y, f, norm);
+        const float x[8] = {a[k].x, a[k].y, a[k].z, a[k].w, b[k].x, b[k].y, b[k].z, b[k].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = f == 0.f && !isfinite(x[e]) ? y[e] + x[e] : fmaf(x[e], f, y[e]);
+      }
     }
     const float inv = norm == 0.f ? 0.f : 1.f / norm;
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] *= inv;
-    const int token = r / p.group, qh = run.head * p.group + r % p.group;
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + d) =
+    const int token = run.q0 + r / p.group, qh = run.head * p.group + r % p.group;
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + token * p.o_ts + qh * p.o_hs + d) =
         make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
     if (d == 0 && p.lse)
-      p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
+      p.lse[static_cast<int64_t>(token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
   }
 }
 

@@ -16,6 +16,7 @@ PyTorch fallback for any of them.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -386,90 +387,75 @@ DTYPE_F16 = 0
 DTYPE_BF16 = 1
 ATTENTION_BAD_PAGE = 1  # attention_status bits
 ATTENTION_TIMEOUT = 2
-_DESC_BYTES = ctypes.sizeof(_native.AexrtB200AttentionDesc)
+# AexrtB200AttentionDesc as bytes: packing takes a fraction of filling the ctypes structure field by field, and
+# these calls are short
+_DESC = struct.Struct("@9If4I10Q")
+assert _DESC.size == ctypes.sizeof(_native.AexrtB200AttentionDesc)
 
 
-def _dtype16(t, what: str) -> int:
-    torch = _torch()
-    if t.dtype == torch.float16:
-        return DTYPE_F16
-    if t.dtype == torch.bfloat16:
+def _dtype16(t, what: str, torch) -> int:
+    dtype = t.dtype
+    if dtype is torch.bfloat16:
         return DTYPE_BF16
-    raise ValueError(f"{what}: float16 or bfloat16 tensors, not {t.dtype}")
+    if dtype is torch.float16:
+        return DTYPE_F16
+    raise ValueError(f"{what}: float16 or bfloat16 tensors, not {dtype}")
 
 
-def _heads(t, what: str, name: str, dims: int = 3):
-    """Checks a [..., heads, head_dim] tensor's rank and its contiguous last dimension."""
-    if t.dim() != dims:
+def _heads(t, what: str, name: str, dims: int):
+    """Shape and strides of a [..., heads, head_dim] tensor with contiguous heads.  A dimension of size 1, whose stride
+    torch leaves arbitrary, counts one row."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != dims:
         raise ValueError(f"{what}: {name} must have {dims} dimensions")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what}: each head of {name} must be contiguous")
+    if 1 in shape:
+        row = max(8, shape[-1])
+        strides = tuple(row if n == 1 else s for n, s in zip(shape, strides))
+    return shape, strides
 
 
-def _index(t, what: str, name: str, size: int) -> int:
+def _index(t, what: str, name: str, size: int, int32) -> int:
     """Checks a contiguous int32 vector and returns its address."""
-    if t.dtype != _torch().int32 or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+    if t.dtype is not int32 or t.dim() != 1 or t.numel() != size or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of {size} entries")
     return t.data_ptr()
 
 
-def _on_device(what: str, first, *others):
-    """Every tensor on `first`'s CUDA device; a guard that makes it current for the call, or None when it is."""
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError(f"{what}: CUDA tensors")
-    for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
-    torch = _torch()
-    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _table(t, what: str, rows: int, int32):
+    """Checks a block table and returns (address, columns, stride of its rows)."""
+    shape, strides = t.shape, t.stride()
+    if t.dtype is not int32 or len(shape) != 2 or shape[0] != rows or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what}: block_table must be int32 [{rows}, columns] with contiguous rows")
+    return t.data_ptr(), shape[1], strides[0] if rows > 1 else shape[1]
 
 
-def _outputs(what: str, q, out, lse, return_lse):
-    torch = _torch()
+def _call(fn, what: str, torch, tensors, stream, args):
+    """Calls a C entry point on the tensors' device (which must be one CUDA device) with `args` and the stream."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or index < 0):
+            raise ValueError(f"{what}: CUDA tensors on one device, not on {tensors[0].device} and {t.device}")
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _call(fn, what, torch, tensors, stream, args)
+    # the current stream's handle as torch keeps it, without a Stream object around it (3 us)
+    handle = torch._C._cuda_getCurrentRawStream(index) if stream is None else _stream(stream)
+    return fn(*args, handle)
+
+
+def _outputs(what: str, torch, q, out, lse, return_lse):
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+    elif out.shape != q.shape or out.dtype is not q.dtype:
         raise ValueError(f"{what}: out must have q's shape and type")
-    _heads(out, what, "out")
     if lse is None:
         if return_lse:
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+    elif lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor [tokens, heads]")
     return out, lse
-
-
-def _stride(t, dim: int) -> int:
-    """A stride that is used: dimensions of size 1 (whose stride torch leaves arbitrary) count 8."""
-    return t.stride(dim) if t.shape[dim] > 1 else max(8, t.shape[-1])
-
-
-def _desc(what, q, k, v, out, num_seqs, max_q, causal, scale):
-    for t, name in ((k, "k"), (v, "v")):
-        if t.dtype != q.dtype or t.shape[-1] != q.shape[-1]:
-            raise ValueError(f"{what}: {name} must have q's type and head size")
-    if k.shape != v.shape:
-        raise ValueError(f"{what}: k and v must have one shape")
-    paged = k.dim() == 4
-    d = _native.AexrtB200AttentionDesc()
-    d.struct_size = _DESC_BYTES
-    d.dtype = _dtype16(q, what)
-    d.num_seqs = num_seqs
-    d.q_tokens, d.q_heads, d.head_dim = q.shape
-    d.max_q = max_q
-    d.kv_heads = k.shape[-2]
-    d.causal = 1 if causal else 0
-    d.scale = q.shape[-1] ** -0.5 if scale is None else scale
-    d.kv_tokens = k.shape[0]
-    if paged:
-        d.page_size = k.shape[1]
-        d.k_page_stride, d.v_page_stride = _stride(k, 0), _stride(v, 0)
-    d.q_token_stride, d.q_head_stride = _stride(q, 0), _stride(q, 1)
-    d.out_token_stride, d.out_head_stride = (_stride(out, 0), _stride(out, 1)) if out is not None else (q.shape[1] * q.shape[2], q.shape[2])
-    d.k_token_stride, d.k_head_stride = _stride(k, -3), _stride(k, -2)
-    d.v_token_stride, d.v_head_stride = _stride(v, -3), _stride(v, -2)
-    return d
 
 
 def attention_packed(q, k, v, cu_q, cu_k, causal: bool = True, scale: Optional[float] = None, out=None, lse=None,
@@ -479,38 +465,36 @@ def attention_packed(q, k, v, cu_q, cu_k, causal: bool = True, scale: Optional[f
     cu_k[s] .. cu_k[s + 1] (int32 on the device).  Causal: the last query token sees every key of its
     sequence.  ``scale`` defaults to d ** -0.5.  Returns out, or (out, lse) with ``return_lse`` or a
     given ``lse`` (fp32 [q_tokens, q_heads], natural logarithm).  Rows behind the last sequence are left as they were."""
-    what = "attention_packed"
-    _heads(q, what, "q")
-    _heads(k, what, "k")
-    _heads(v, what, "v")
-    out, lse = _outputs(what, q, out, lse, return_lse)
-    guard = _on_device(what, q, k, v, cu_q, cu_k, out, lse)
+    what, torch = "attention_packed", _torch()
+    (tokens, heads, dim), qs = _heads(q, what, "q", 3)
+    k_shape, ks = _heads(k, what, "k", 3)
+    v_shape, vs = _heads(v, what, "v", 3)
+    out, lse = _outputs(what, torch, q, out, lse, return_lse)
+    _, os_ = _heads(out, what, "out", 3)
+    if k_shape != v_shape or k_shape[2] != dim or not q.dtype is k.dtype is v.dtype:
+        raise ValueError(f"{what}: k and v must have one shape, and q's type and head size")
     num_seqs = cu_q.shape[0] - 1
     if num_seqs < 0:
         raise ValueError(f"{what}: cu_q must have at least one entry")
-    d = _desc(what, q, k, v, out, num_seqs, 0, causal, scale)
-    args = (ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), _index(cu_q, what, "cu_q", num_seqs + 1),
-            _index(cu_k, what, "cu_k", num_seqs + 1), out.data_ptr(), _ptr(lse))
-    if guard is None:
-        check(_native.load().aexrt_b200_attention_packed(*args, _stream(stream)), what)
-    else:
-        with guard:
-            check(_native.load().aexrt_b200_attention_packed(*args, _stream(stream)), what)
+    desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, 0, heads, k_shape[1], dim, 1 if causal else 0,
+                      dim ** -0.5 if scale is None else scale, k_shape[0], 0, 0, 0, qs[0], qs[1], os_[0], os_[1],
+                      ks[0], ks[1], 0, vs[0], vs[1], 0)
+    check(_call(_native.load().aexrt_b200_attention_packed, what, torch, (q, k, v, cu_q, cu_k, out, lse), stream,
+                (desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), _index(cu_q, what, "cu_q", num_seqs + 1, torch.int32),
+                 _index(cu_k, what, "cu_k", num_seqs + 1, torch.int32), out.data_ptr(), _ptr(lse))), what)
     return out if lse is None else (out, lse)
 
 
 def attention_paged_workspace(q, k_cache, num_seqs: int, max_q: int):
     """A workspace tensor for :func:`attention_paged` calls of these shapes (any lengths and tables).  Calls that can
     overlap on the GPU each need their own."""
-    torch = _torch()
-    guard = _on_device("attention_paged", q, k_cache)
-    d = _desc("attention_paged", q, k_cache, k_cache, None, num_seqs, max_q, True, None)
-    if guard is None:
-        n = _native.load().aexrt_b200_attention_paged_workspace(ctypes.byref(d))
-    else:
-        with guard:
-            n = _native.load().aexrt_b200_attention_paged_workspace(ctypes.byref(d))
-    check(n != 2 ** 64 - 1, "attention_paged_workspace")
+    what, torch = "attention_paged", _torch()
+    (tokens, heads, dim), qs = _heads(q, what, "q", 3)
+    k_shape, ks = _heads(k_cache, what, "k_cache", 4)
+    desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1, 1.0, k_shape[0],
+                      k_shape[1], 0, 0, qs[0], qs[1], heads * dim, dim, ks[1], ks[2], ks[0], ks[1], ks[2], ks[0])
+    n = _call(lambda desc, stream: _native.load().aexrt_b200_attention_paged_workspace(desc), what, torch, (q, k_cache), 0, (desc,))
+    check(n != 2 ** 64 - 1, what)
     return torch.empty((n,), dtype=torch.uint8, device=q.device)
 
 
@@ -522,32 +506,28 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
     a power of two from 8 to 1024), ``block_table`` [num_seqs, columns] int32, ``kv_lens`` [num_seqs] int32: cached keys
     of each sequence, the new tokens' own among them (see :func:`page_tables` and :func:`kv_append`).  ``workspace``:
     from :func:`attention_paged_workspace`; without one the call allocates it."""
-    what = "attention_paged"
-    torch = _torch()
-    _heads(q, what, "q")
-    _heads(k_cache, what, "k_cache", 4)
-    _heads(v_cache, what, "v_cache", 4)
-    out, lse = _outputs(what, q, out, lse, return_lse)
-    guard = _on_device(what, q, k_cache, v_cache, block_table, cu_q, kv_lens, out, lse, workspace)
+    what, torch = "attention_paged", _torch()
+    (tokens, heads, dim), qs = _heads(q, what, "q", 3)
+    k_shape, ks = _heads(k_cache, what, "k_cache", 4)
+    v_shape, vs = _heads(v_cache, what, "v_cache", 4)
+    out, lse = _outputs(what, torch, q, out, lse, return_lse)
+    _, os_ = _heads(out, what, "out", 3)
+    if k_shape != v_shape or k_shape[3] != dim or not q.dtype is k_cache.dtype is v_cache.dtype:
+        raise ValueError(f"{what}: the caches must have one shape, and q's type and head size")
     num_seqs = kv_lens.shape[0]
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != num_seqs or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"{what}: block_table must be int32 [{num_seqs}, columns] with contiguous rows")
-    d = _desc(what, q, k_cache, v_cache, out, num_seqs, max_q, causal, scale)
-    d.table_columns = block_table.shape[1]
-    d.table_stride = block_table.stride(0) if num_seqs > 1 else block_table.shape[1]
+    table, columns, table_stride = _table(block_table, what, num_seqs, torch.int32)
     if workspace is None:
         workspace = attention_paged_workspace(q, k_cache, num_seqs, max_q)
     elif not workspace.is_contiguous():
         raise ValueError(f"{what}: workspace must be contiguous")
-    args = (ctypes.byref(d), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-            _index(cu_q, what, "cu_q", num_seqs + 1), _index(kv_lens, what, "kv_lens", num_seqs), out.data_ptr(),
-            _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    if guard is None:
-        check(_native.load().aexrt_b200_attention_paged(*args, _stream(stream)), what)
-    else:
-        with guard:
-            check(_native.load().aexrt_b200_attention_paged(*args, _stream(stream)), what)
+    desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1 if causal else 0,
+                      dim ** -0.5 if scale is None else scale, k_shape[0], k_shape[1], columns, table_stride,
+                      qs[0], qs[1], os_[0], os_[1], ks[1], ks[2], ks[0], vs[1], vs[2], vs[0])
+    check(_call(_native.load().aexrt_b200_attention_paged, what, torch,
+                (q, k_cache, v_cache, block_table, cu_q, kv_lens, out, lse, workspace), stream,
+                (desc, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table,
+                 _index(cu_q, what, "cu_q", num_seqs + 1, torch.int32), _index(kv_lens, what, "kv_lens", num_seqs, torch.int32), out.data_ptr(),
+                 _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size())), what)
     return out if lse is None else (out, lse)
 
 
@@ -567,13 +547,11 @@ def page_tables(ctx_lens, new_lens, block_table, free_pages, free_state, page_si
     slot_map [max_tokens], free_state_out [2] = new top and pages missing), all int32.  slot_map holds each new
     token's slot, -1 where it has no page and behind the last token.  ``kv_lens`` may be ``ctx_lens`` and
     ``free_state_out`` may be ``free_state``: updated in place, as a captured step wants them."""
-    what = "page_tables"
-    torch = _torch()
+    what, torch = "page_tables", _torch()
     n = ctx_lens.shape[0]
-    dev = ctx_lens.device
 
     def ints(size):
-        return torch.empty((size,), dtype=torch.int32, device=dev)
+        return torch.empty((size,), dtype=torch.int32, device=ctx_lens.device)
 
     if slot_map is None:
         if max_tokens is None:
@@ -582,23 +560,14 @@ def page_tables(ctx_lens, new_lens, block_table, free_pages, free_state, page_si
     cu_q = ints(n + 1) if cu_q is None else cu_q
     kv_lens = ints(n) if kv_lens is None else kv_lens
     free_state_out = ints(2) if free_state_out is None else free_state_out
-    guard = _on_device(what, ctx_lens, new_lens, block_table, free_pages, free_state, cu_q, kv_lens, slot_map,
-                       free_state_out)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"{what}: block_table must be int32 [{n}, columns] with contiguous rows")
-    columns = block_table.shape[1]
-    stride = block_table.stride(0) if n > 1 else columns
-    args = (_index(ctx_lens, what, "ctx_lens", n), _index(new_lens, what, "new_lens", n), n, page_size,
-            block_table.data_ptr(), columns, stride, _index(free_pages, what, "free_pages", free_pages.shape[0]),
-            free_pages.shape[0], _index(free_state, what, "free_state", 2),
-            _index(free_state_out, what, "free_state_out", 2), _index(cu_q, what, "cu_q", n + 1),
-            _index(kv_lens, what, "kv_lens", n), _index(slot_map, what, "slot_map", slot_map.shape[0]), slot_map.shape[0])
-    if guard is None:
-        check(_native.load().aexrt_b200_page_tables(*args, _stream(stream)), what)
-    else:
-        with guard:
-            check(_native.load().aexrt_b200_page_tables(*args, _stream(stream)), what)
+    table, columns, table_stride = _table(block_table, what, n, torch.int32)
+    free, slots = free_pages.shape[0], slot_map.shape[0]
+    check(_call(_native.load().aexrt_b200_page_tables, what, torch,
+                (ctx_lens, new_lens, block_table, free_pages, free_state, cu_q, kv_lens, slot_map, free_state_out), stream,
+                (_index(ctx_lens, what, "ctx_lens", n, torch.int32), _index(new_lens, what, "new_lens", n, torch.int32), n, page_size, table, columns,
+                 table_stride, _index(free_pages, what, "free_pages", free, torch.int32), free, _index(free_state, what, "free_state", 2, torch.int32),
+                 _index(free_state_out, what, "free_state_out", 2, torch.int32), _index(cu_q, what, "cu_q", n + 1, torch.int32),
+                 _index(kv_lens, what, "kv_lens", n, torch.int32), _index(slot_map, what, "slot_map", slots, torch.int32), slots)), what)
     return cu_q, kv_lens, slot_map, free_state_out
 
 
@@ -606,25 +575,17 @@ def kv_append(k, v, slot_map, k_cache, v_cache, stream=None):
     """Writes rows ``k``, ``v`` [tokens, kv_heads, d] to their slots (page * page_size + row) of the paged caches
     [pages, page_size, kv_heads, d], in place; slots outside the cache (-1) are skipped.  Slots of one call are
     distinct, or each 16-byte piece of a shared slot comes from one of its tokens."""
-    what = "kv_append"
-    _heads(k, what, "k")
-    _heads(v, what, "v")
-    _heads(k_cache, what, "k_cache", 4)
-    _heads(v_cache, what, "v_cache", 4)
-    _dtype16(k, what)
-    if k.shape != v.shape or k_cache.shape != v_cache.shape or k.shape[1:] != k_cache.shape[2:]:
+    what, torch = "kv_append", _torch()
+    k_shape, ks = _heads(k, what, "k", 3)
+    v_shape, vs = _heads(v, what, "v", 3)
+    kc_shape, kcs = _heads(k_cache, what, "k_cache", 4)
+    vc_shape, vcs = _heads(v_cache, what, "v_cache", 4)
+    _dtype16(k, what, torch)
+    if k_shape != v_shape or kc_shape != vc_shape or k_shape[1:] != kc_shape[2:]:
         raise ValueError(f"{what}: k and v, and the caches, must agree in heads and head size")
-    if not k.dtype == v.dtype == k_cache.dtype == v_cache.dtype:
+    if not k.dtype is v.dtype is k_cache.dtype is v_cache.dtype:
         raise ValueError(f"{what}: one type for k, v and the caches")
-    guard = _on_device(what, k, v, slot_map, k_cache, v_cache)
-    tokens, heads, dim = k.shape
-    pages, page = k_cache.shape[:2]
-    args = (k.data_ptr(), v.data_ptr(), tokens, heads, dim, _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1),
-            _index(slot_map, what, "slot_map", tokens), k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
-            _stride(k_cache, 0), _stride(k_cache, 1), _stride(k_cache, 2), _stride(v_cache, 0), _stride(v_cache, 1),
-            _stride(v_cache, 2))
-    if guard is None:
-        check(_native.load().aexrt_b200_kv_append(*args, _stream(stream)), what)
-    else:
-        with guard:
-            check(_native.load().aexrt_b200_kv_append(*args, _stream(stream)), what)
+    check(_call(_native.load().aexrt_b200_kv_append, what, torch, (k, v, slot_map, k_cache, v_cache), stream,
+                (k.data_ptr(), v.data_ptr(), k_shape[0], k_shape[1], k_shape[2], ks[0], ks[1], vs[0], vs[1],
+                 _index(slot_map, what, "slot_map", k_shape[0], torch.int32), k_cache.data_ptr(), v_cache.data_ptr(), kc_shape[0],
+                 kc_shape[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2])), what)
