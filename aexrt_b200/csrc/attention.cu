@@ -129,8 +129,9 @@ bool desc_ok(const AexrtB200AttentionDesc* d, bool paged) {
   if (paged) {
     if (d->page_size < 8 || d->page_size > 1024 || (d->page_size & (d->page_size - 1)))
       return fail("%s: page_size must be a power of two from 8 to 1024", what) != 0;
-    if (d->table_columns > (1u << 30) || d->table_stride < d->table_columns)
-      return fail("%s: table_stride below table_columns", what) != 0;
+    if (d->table_stride < d->table_columns) return fail("%s: table_stride below table_columns", what) != 0;
+    if (static_cast<uint64_t>(d->table_columns) * d->page_size > (1ull << 30))
+      return fail("%s: a table row of more than 2^30 tokens", what) != 0;
   }
   return true;
 }
@@ -255,10 +256,10 @@ int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, 
   if (!kv_maps(d, p, paged, kTcTileKeys, maps + 1)) return 0;
   const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, p.head_dim);
   if (!raise_smem(reinterpret_cast<const void*>(k.fn), k.smem)) return 0;
-  // every sequence ends in at most one partial pair of tiles
-  const uint64_t blocks = (static_cast<uint64_t>(d->q_tokens) / (2 * tokens) + d->num_seqs) * d->kv_heads;
-  if (blocks >= (1ull << 31)) return fail("attention: %llu blocks exceed the grid", static_cast<unsigned long long>(blocks));
-  return cuda_ok(launch_kernel(k.fn, dim3(static_cast<unsigned>(blocks)), dim3(kTcBlock), k.smem, st, maps[0], maps[1],
+  // one block per SM, fewer when there cannot be an item for each: every sequence ends in at most one partial pair of tiles
+  const uint64_t items = (static_cast<uint64_t>(d->q_tokens) / (2 * tokens) + d->num_seqs) * d->kv_heads;
+  const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(items, sm_count()));
+  return cuda_ok(launch_kernel(k.fn, dim3(blocks), dim3(kTcBlock), k.smem, st, maps[0], maps[1],
                                maps[2], p),
                  "attention launch")
              ? 1

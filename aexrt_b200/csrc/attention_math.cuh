@@ -15,6 +15,12 @@ __device__ __forceinline__ float exp2_sfu(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi);
 template <>
@@ -38,27 +44,29 @@ __device__ __forceinline__ uint32_t non_finite_bits(uint32_t w) {
                                      : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
-// Kind of a non-finite 16-bit value: 0 +inf, 1 -inf, 2 NaN.
+// Notes a non-finite value (bits h) of column `col` of key `key`: fix[col] has the first key with +inf or
+// NaN, fix[128 + col] the first with -inf or NaN.
 template <typename T>
-__device__ __forceinline__ int non_finite_kind(uint32_t h) {
-  const uint32_t mantissa = __is_same(T, __nv_bfloat16) ? h & 0x7fu : h & 0x3ffu;
-  return mantissa ? 2 : static_cast<int>(h >> 15) & 1;
+__device__ __forceinline__ void note_non_finite(uint32_t h, int key, int col, int* fix) {
+  const bool nan = (h & (__is_same(T, __nv_bfloat16) ? 0x7fu : 0x3ffu)) != 0, down = (h >> 15) & 1;
+  if (nan || !down) atomicMin(fix + col, key);
+  if (nan || down) atomicMin(fix + 128 + col, key);
 }
 
 // Takes the non-finite values out of 16 bytes of a V tile (values of columns d0 .. d0 + 7 of key
-// `key`): zeros in their place, and the first such key of each column and kind in fix.
+// `key`): zeros in their place, and a note of them.
 template <typename T>
-__device__ __noinline__ uint4 take_non_finite(uint4 x, int key, int d0, int* fix) {
+__device__ __forceinline__ uint4 take_non_finite(uint4 x, int key, int d0, int* fix) {
   uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t b = non_finite_bits<T>(w[i]);
     if (b & 0x8000u) {
-      atomicMin(fix + non_finite_kind<T>(w[i] & 0xffffu) * 128 + d0 + 2 * i, key);
+      note_non_finite<T>(w[i] & 0xffffu, key, d0 + 2 * i, fix);
       w[i] &= 0xffff0000u;
     }
     if (b & 0x80000000u) {
-      atomicMin(fix + non_finite_kind<T>(w[i] >> 16) * 128 + d0 + 2 * i + 1, key);
+      note_non_finite<T>(w[i] >> 16, key, d0 + 2 * i + 1, fix);
       w[i] &= 0xffffu;
     }
   }
@@ -67,9 +75,9 @@ __device__ __noinline__ uint4 take_non_finite(uint4 x, int key, int d0, int* fix
 
 // What a row that sees keys 0 .. seen - 1 gets in a column from values that were taken out.
 __device__ __forceinline__ float put_back(float o, const int* fix, int col, int seen) {
-  const bool up = fix[col] < seen, down = fix[128 + col] < seen, nan = fix[256 + col] < seen;
-  if (nan || (up && down)) return __int_as_float(0x7fffffff);
-  return up ? INFINITY : (down ? -INFINITY : o);
+  const bool up = fix[col] < seen, down = fix[128 + col] < seen;
+  return up ? (down ? __int_as_float(0x7fffffff) : INFINITY) : (down ? -INFINITY : o);
 }
+constexpr int kFixInts = 2 * 128;
 
 }  // namespace aexrt

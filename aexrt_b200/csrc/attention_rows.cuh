@@ -33,7 +33,7 @@ struct RowsSmem {
   static_assert(kStage == 4 * 16 * DP * 4, "a stage holds the four warps' accumulators");
   static constexpr int kStat = rows_stages<DP>() * kStage;              // m, l of each warp's rows
   static constexpr int kFix = kStat + 4 * 16 * 2 * 4;
-  static constexpr int kBars = kFix + 3 * 128 * 4 + 16;
+  static constexpr int kBars = kFix + kFixInts * 4 + 16;
   static constexpr int kBytes = kBars + 2 * rows_stages<DP>() * 8;
 };
 
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   const AttnParams& p = rp.a;
   float* stat = reinterpret_cast<float*>(smem + L::kStat);
   int* fix = reinterpret_cast<int*>(smem + L::kFix);
-  int* fixed = fix + 3 * 128;
+  int* fixed = fix + kFixInts;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* empty = full + kStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   grid_dep_wait();
 
   // ---- this CTA's run: the units of every sequence are summed, then the one that holds the first unit found
-  for (int i = tid; i < 3 * 128; i += kRowsThreads) fix[i] = INT_MAX;
+  for (int i = tid; i < kFixInts; i += kRowsThreads) fix[i] = INT_MAX;
   if (tid == 0) *fixed = 0;
   constexpr int kWarps = kRowsThreads / 32;
   __shared__ int64_t sums[kWarps];
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       }
       if (patch) {
         named_bar_sync(1, kRowsCompute);
-        for (int i = tid; i < 3 * 128; i += kRowsCompute) fix[i] = INT_MAX;
+        for (int i = tid; i < kFixInts; i += kRowsCompute) fix[i] = INT_MAX;
         if (tid == 0) *fixed = 0;
       }
       fence_proxy_async_smem();      // these accesses before the stage's next TMA write

@@ -1,20 +1,33 @@
 // Attention of many query rows on the tensor cores: packed prompts, and chunks of new tokens over
 // the paged cache.
 //
-// One CTA takes two tiles of 128 query rows of one key/value head (rows: token x the query heads that
-// share the head, so grouped heads read each key tile once) and walks the keys that they see in
+// A work item is two tiles of 128 query rows of one key/value head (rows: token x the query heads that
+// share the head, so grouped heads read each key tile once), walked over the keys that they see in
 // tiles of 128.  Per tile and key tile: S = Q K^T into TMEM, the softmax warps turn S into
-// probabilities P, which replace S in TMEM as 16-bit pairs, and O += P V with P as the TMEM operand.
+// probabilities P, 16-bit pairs in TMEM, and O += P V with P as the TMEM operand.
 // Two row tiles share every K and V tile, so that the tensor core works on one while the softmax
-// warps work on the other.  A thread owns a row, so the running maximum m and sum l need no exchange
+// warps work on the other.  S has one place in TMEM, which the tiles take in turn: a tile's scores leave it for
+// registers at once, so the next product needs neither to wait for the exponentials nor for P to be consumed
+// (with P in S's place each tile's P V, the next S and their latency, 1400 clocks, followed the 1850 of its
+// softmax: 1040 TFLOP/s).  A thread owns a row, so the running maximum m and sum l need no exchange
 // between threads.  O in TMEM is in units of a reference maximum that moves only when a row's true
 // maximum has passed it by 2^8: P stays below 2^8 (far inside fp16) and the rescaling of O, a
 // round trip through registers, is skipped for almost every tile.
 //
-// Roles: warps 0-3 softmax of tile 0, warps 4-7 of tile 1, warp 8 (one thread) issues the MMAs, warp 9
-// loads, warps 10 and 11 only complete the third warpgroup: registers are split by warpgroup, 216 for a softmax thread
-// (it holds a whole row of S) and 72 for the others, 2 * 216 + 72 = 3 * 168 as launched.
-// TMEM columns: S0 0-127, S1 128-255, O0 256-, O1 384-.
+// A 128 x 128 tile costs 1024 clocks of exp on the special-function units (16 a clock), as many as its
+// two products at head size 128.  Taking a part of the powers by a polynomial on the multiply-add
+// pipes instead made every size slower (8 of 32: 3 %, 16 of 32: 8 %): the softmax warps are not what the products wait for.
+//
+// One CTA per SM stays for all its items: the loads, the score products and the search of the next
+// item go on while the softmax warps write the last one's output.  Items go out in the order of their key tiles,
+// the longest first, so that ragged batches and the causal triangle end evenly.
+//
+// Roles: warps 0-3 softmax of tile 0, warps 4-7 of tile 1, one thread each of warps 8 and 11 issues
+// the MMAs of tile 0 and of tile 1 (one thread for both spent 93 clocks an MMA instead of the
+// pipe's 64: it holds few MMAs, and ran dry whenever the thread looked at its barriers), warp 9
+// loads, warp 10 finds the items.  Registers are split by warpgroup, 216 for a softmax thread (it
+// holds a whole row of S) and 72 for the others, 2 * 216 + 72 = 3 * 168 as launched.
+// TMEM columns: S 0-127, P0 128-191, P1 192-255, O0 256-, O1 384-.
 #pragma once
 #include <climits>
 
@@ -34,8 +47,8 @@ template <int DP>
 struct TcSmem {
   static constexpr int kTile = 128 * DP * 2;
   static constexpr int kQ = 0, kRing = 2 * kTile, kBars = kRing + tc_slots<DP>() * kTile;
-  // barriers, TMEM base, flags, then the first key with a +inf, -inf or NaN in a value column
-  static constexpr int kFix = kBars + 256, kBytes = kFix + 3 * 128 * 4;
+  // barriers, TMEM base, items; then, per item of two, the first keys with non-finite values of a column
+  static constexpr int kFix = kBars + 512, kBytes = kFix + 2 * kFixInts * 4;
 };
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -70,49 +83,163 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t* r)
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
+// 16 columns: the rescaling runs beside a whole row of S in registers.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::
+          "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 struct TcWork {
-  int seq, tile, len_q, rows_q, len_k, q0, k0;  // rows_q: query tokens taken (len_q, at most max_q)
+  int head, seq, tile, len_q, rows_q, len_k, q0, k0;  // rows_q: query tokens taken (len_q, at most max_q); head -1: no more
 };
 
-// The work item that is number `w` when every sequence has ceil(rows / tokens) of them; false past the end.
+// Numbers the items of a call: descending in key tiles while a warp can hold every sequence's lengths
+// (kHeld per lane), else by sequence.  Asked for ascending numbers, by a whole warp.
 template <bool kPaged>
-__device__ __forceinline__ bool tc_find(const AttnParams& p, int64_t w, int tokens, TcWork& out) {
-  const int lane = threadIdx.x & 31;
+struct TcFinder {
+  static constexpr int kHeld = 4;
+  const AttnParams& p;
+  int tokens;  // query tokens of an item
+  int rows[kHeld], shift[kHeld], tiles[kHeld];  // of sequence 32 * h + lane: rows, len_k - len_q, key tiles of the last item
+  int base = 0;      // by sequence: the first sequence of the 32 looked at, and the items before it
   int64_t before = 0;
-  for (int base = 0; base < p.num_seqs; base += 32) {
-    const int s = base + lane;
-    int rows = 0;
-    if (s < p.num_seqs) {
-      rows = q_len(p, s);
-      if (kPaged) rows = min(rows, p.max_q);
-    }
-    const int n = (rows + tokens - 1) / tokens;
-    int sum = n;
+
+  __device__ __forceinline__ TcFinder(const AttnParams& params, int tokens_) : p(params), tokens(tokens_) {
+    if (p.num_seqs <= 32 * kHeld) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int z = __shfl_up_sync(~0u, sum, o);
-      if (lane >= o) sum += z;
+      for (int h = 0; h < kHeld; ++h) {
+        const int s = 32 * h + (threadIdx.x & 31);
+        rows[h] = shift[h] = tiles[h] = 0;
+        if (s < p.num_seqs) {
+          const int len_k = k_len<kPaged>(p, s);
+          rows[h] = rows_of(s);
+          shift[h] = len_k - q_len(p, s);
+          tiles[h] = rows[h] ? (keys_seen(rows[h] - 1, q_len(p, s), len_k, p.causal) + kTcKeys - 1) / kTcKeys : 0;
+        }
+      }
     }
-    const uint32_t past = __ballot_sync(~0u, before + sum > w);
-    if (past) {
-      const int src = __ffs(past) - 1;
-      out.seq = base + src;
-      const int tiles = __shfl_sync(~0u, n, src);
-      const int first = __shfl_sync(~0u, sum - n, src);
-      out.rows_q = __shfl_sync(~0u, rows, src);
-      // the last tiles of a causal sequence see the most keys: they go first
-      out.tile = tiles - 1 - static_cast<int>(w - before - first);
-      out.len_q = q_len(p, out.seq);
-      out.q0 = q_start(p, out.seq);
-      out.len_k = k_len<kPaged>(p, out.seq);
-      out.k0 = k_start<kPaged>(p, out.seq);
-      return true;
-    }
-    before += __shfl_sync(~0u, sum, 31);
   }
-  return false;
+  __device__ __forceinline__ int rows_of(int s) const { return kPaged ? min(q_len(p, s), p.max_q) : q_len(p, s); }
+  // Items of held sequence h of this lane with at least `level` key tiles.
+  __device__ __forceinline__ int items_from(int h, int level) const {
+    const int all = (rows[h] + tokens - 1) / tokens;
+    if (level <= 0) return all;
+    if (level > tiles[h]) return 0;
+    if (!p.causal) return all;
+    // item t ends at token e = min((t + 1) * tokens, rows) and sees e + shift keys
+    const int e = (level - 1) * kTcKeys + 1 - shift[h];
+    return e <= 0 ? all : all - (e + tokens - 1) / tokens + 1;
+  }
+  __device__ __forceinline__ int64_t all_from(int level) const {
+    int64_t n = 0;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+      if (32 * h < p.num_seqs) n += items_from(h, level);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
+    return n;
+  }
+  __device__ __forceinline__ void fill(TcWork& w, int s, int tile) const {
+    w.seq = s;
+    w.tile = tile;
+    w.rows_q = rows_of(s);
+    w.len_q = q_len(p, s);
+    w.q0 = q_start(p, s);
+    w.len_k = k_len<kPaged>(p, s);
+    w.k0 = k_start<kPaged>(p, s);
+  }
+  __device__ __forceinline__ bool find(int64_t item, TcWork& w) {
+    const int lane = threadIdx.x & 31;
+    if (p.num_seqs <= 32 * kHeld) {
+      if (item >= all_from(0)) return false;
+      int lo = 0, hi = 0;  // the highest level that has more than `item` items at or above it
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) hi = max(hi, tiles[h]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) hi = max(hi, __shfl_xor_sync(~0u, hi, o));
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (all_from(mid) > item) lo = mid; else hi = mid - 1;
+      }
+      int64_t rank = item - all_from(lo + 1);  // among the items of exactly this level
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        if (32 * h >= p.num_seqs) break;
+        const int above = items_from(h, lo + 1), n = items_from(h, lo) - above;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int z = __shfl_up_sync(~0u, sum, o);
+          if (lane >= o) sum += z;
+        }
+        const uint32_t past = __ballot_sync(~0u, sum > rank);
+        if (past) {
+          const int src = __ffs(past) - 1;
+          const int all = (rows[h] + tokens - 1) / tokens;
+          // a sequence's later items see more keys: those above this level are its last ones
+          const int tile = all - 1 - above - static_cast<int>(rank - (sum - n));
+          fill(w, 32 * h + src, __shfl_sync(~0u, tile, src));
+          return true;
+        }
+        rank -= __shfl_sync(~0u, sum, 31);
+      }
+      return false;
+    }
+    for (; base < p.num_seqs; base += 32) {
+      const int s = base + lane;
+      const int n = s < p.num_seqs ? (rows_of(s) + tokens - 1) / tokens : 0;
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(~0u, sum, o);
+        if (lane >= o) sum += z;
+      }
+      const uint32_t past = __ballot_sync(~0u, before + sum > item);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        const int tile = n - 1 - static_cast<int>(item - before - (sum - n));
+        fill(w, base + src, __shfl_sync(~0u, tile, src));
+        return true;
+      }
+      before += __shfl_sync(~0u, sum, 31);
+    }
+    return false;
+  }
+};
+
+// An item's two row tiles: first token, tokens, keys that the last one sees, key tiles.
+struct TcTiles {
+  int first[2], valid[2], n[2];
+  int key_end, nmax, common;  // keys at and above `common` are seen by some rows and not by others
+  __device__ __forceinline__ TcTiles(const AttnParams& p, const TcWork& w, int tokens) {
+    int keys[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      first[s] = (w.tile * 2 + s) * tokens;
+      valid[s] = clampi(w.rows_q - first[s], 0, tokens);
+      keys[s] = valid[s] ? keys_seen(first[s] + valid[s] - 1, w.len_q, w.len_k, p.causal) : 0;
+      n[s] = (keys[s] + kTcKeys - 1) / kTcKeys;
+    }
+    key_end = max(keys[0], keys[1]);
+    nmax = max(n[0], n[1]);
+    common = min(keys_seen(first[0], w.len_q, w.len_k, p.causal), key_end);
+  }
+};
+
+__device__ __forceinline__ void mbar_arrive_count(uint64_t* bar, uint32_t count) {
+  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(smem_u32(bar)), "r"(count)
+               : "memory");
 }
 
 template <int kRegs>
@@ -128,134 +255,160 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   using L = TcSmem<DP>;
   constexpr int NS = tc_slots<DP>(), kHalves = DP / 64;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  uint64_t *kv_full = q_full + 2, *kv_empty = kv_full + NS, *raw = kv_empty + NS, *s_full = raw + 1, *p_full = s_full + 2,
-           *o_done = p_full + 2;
-  uint64_t* drain = o_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  int* fixed = reinterpret_cast<int*>(tmem_slot + 1);
-  int* fix = reinterpret_cast<int*>(smem + L::kFix);
-  static_assert((2 + 2 * tc_slots<DP>() + 8) * 8 + 8 <= 256, "barriers fit");
+  uint64_t *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 2, *o_done = p_full + 2, *w_full = o_done + 2,
+           *w_empty = w_full + 2, *kv_full = w_empty + 2, *kv_empty = kv_full + NS, *raw = kv_empty + NS, *s_free = raw + 1,
+           *drain = s_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  int* fixed = reinterpret_cast<int*>(tmem_slot + 1);  // [2]
+  TcWork* work = reinterpret_cast<TcWork*>(fixed + 3);  // [2]
+  int* fix = reinterpret_cast<int*>(smem + L::kFix);    // [2][kFixInts]
+  static_assert((14 + 2 * tc_slots<DP>() + 5) * 8 + 16 + 2 * sizeof(TcWork) <= 512, "barriers and items fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dep_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 128);
       mbar_init(o_done + i, 1);
+      mbar_init(w_full + i, 1);
+      mbar_init(w_empty + i, 11);  // the loading warp, two MMA threads, eight softmax warps
+      mbar_init(s_free + i, 128);
+      mbar_init(drain + i, 1);
+      fixed[i] = 0;
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+      mbar_init(kv_empty + i, 2);
     }
     mbar_init(raw, 1);
-    mbar_init(drain, 1);
     fence_mbar_init();
-    *fixed = 0;
   }
-  for (int i = threadIdx.x; i < 3 * 128; i += kTcThreads) fix[i] = INT_MAX;
+  for (int i = threadIdx.x; i < 2 * kFixInts; i += kTcThreads) fix[i] = INT_MAX;
   if (warp == 8) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   grid_dep_wait();
-  const int tokens = kTcRows / p.group;  // query tokens of a tile
-  const int head = static_cast<int>(blockIdx.x % p.kv_heads);
-  TcWork w;
-  const bool found = tc_find<kPaged>(p, blockIdx.x / p.kv_heads, 2 * tokens, w);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int tokens = kTcRows / p.group;  // query tokens of a row tile
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait_bounded(bar, phase & 1, p.status, kAttnTimeout); };
+  // Item number k of this CTA, once it is known; head -1 ends the roles (so does a wait that gave up).
+  auto item = [&](int k, TcWork& w) {
+    const bool ok = wait(w_full + (k & 1), k >> 1);
+    w = work[k & 1];
+    return ok && w.head >= 0;
+  };
 
-  if (found) {
-    int first[2], valid[2], keys[2], n[2];  // per row tile: first token, tokens, keys seen by the last, key tiles
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      first[s] = w.tile * 2 * tokens + s * tokens;
-      valid[s] = clampi(w.rows_q - first[s], 0, tokens);
-      keys[s] = valid[s] ? keys_seen(first[s] + valid[s] - 1, w.len_q, w.len_k, p.causal) : 0;
-      n[s] = (keys[s] + kTcKeys - 1) / kTcKeys;
-    }
-    const int key_end = max(keys[0], keys[1]), nmax = max(n[0], n[1]);
-    // keys at and above `common` are seen by some rows of the CTA and not by others
-    const int common = min(keys_seen(first[0], w.len_q, w.len_k, p.causal), key_end);
-
-    if (warp >= 8) {
-      regs_down<72>();
-      if (warp == 9) {
+  if (warp >= 8) {
+    regs_down<72>();
+    if (warp == 10) {
+      // ---------------------------------------------------------------- items
+      TcFinder<kPaged> finder(p, 2 * tokens);
+      for (int k = 0;; ++k) {
+        const int64_t number = static_cast<int64_t>(k) * gridDim.x + blockIdx.x;
+        TcWork w = {};
+        const bool found = finder.find(number / p.kv_heads, w);
+        w.head = found ? static_cast<int>(number % p.kv_heads) : -1;
+        if (!__all_sync(~0u, wait(w_empty + (k & 1), (k >> 1) + 1))) break;
+        if (lane == 0) {
+          work[k & 1] = w;
+          mbar_arrive(w_full + (k & 1));
+        }
+        if (!found) break;
+      }
+    } else if (warp == 9) {
       // ---------------------------------------------------------------- loads
       const uint32_t q_bytes = static_cast<uint32_t>(tokens * p.group * 128 * kHalves);
-      auto load_q = [&](int s) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(q_full + s, q_bytes);
-          for (int h = 0; h < kHalves; ++h)
-            tma_load_4d(smem + L::kQ + s * L::kTile + h * 16384, &q_map, q_full + s, h * 64, 0, head, w.q0 + first[s]);
-        }
-      };
-      // one K or V tile; the bytes count whole boxes, what lies outside the tensor arrives as zeros
-      auto load_kv = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
-        if (lane == 0) mbar_arrive_expect_tx(bar, L::kTile);
-        __syncwarp();
-        if constexpr (kPaged) {
-          const int rows = min(1 << p.page_shift, kTcKeys);
-          const int key = j * kTcKeys + lane * rows;
-          if (lane * rows < kTcKeys) {
-            int page = p.kv_tokens;  // outside: zeros
-            if (key < key_end) {
-              const int id = __ldg(p.block_table + w.seq * p.table_stride + (key >> p.page_shift));
-              if (id >= 0 && id < p.kv_tokens) page = id; else atomicOr(p.status, kAttnBadPage);
-            }
-            for (int h = 0; h < kHalves; ++h)
-              tma_load_4d(dst + h * 16384 + lane * rows * 128, map, bar, h * 64, head, key & ((1 << p.page_shift) - 1), page);
-          }
-        } else if (lane == 0) {
-          for (int h = 0; h < kHalves; ++h) tma_load_3d(dst + h * 16384, map, bar, h * 64, head, w.k0 + j * kTcKeys);
-        }
-        __syncwarp();
-      };
       bool ok = true;
-      int raw_phase = 0;
-      if (nmax) load_q(0);
-      for (int i = 0; i < 2 * nmax && ok; ++i) {  // K0 V0 K1 V1 ...
-        const int slot = i % NS, j = i >> 1;
-        uint8_t* dst = smem + L::kRing + slot * L::kTile;
-        ok = mbar_wait_bounded(kv_empty + slot, ((i / NS) & 1) ^ 1, p.status, kAttnTimeout);
-        if (!ok) break;
-        const int last = key_end - j * kTcKeys, seen = common - j * kTcKeys;  // rows of this tile below them
-        const bool clean = (i & 1) && (last < kTcKeys || (seen < kTcKeys && seen < last));
-        load_kv((i & 1) ? &v_map : &k_map, dst, clean ? raw : kv_full + slot, j);
-        if (i == 0 && n[1]) load_q(1);
-        if (clean) {
-          // P is 0 where a row does not see a key, but 0 * inf and 0 * NaN are not: rows behind the
-          // last key become zeros, and non-finite values of keys that only some rows see are taken
-          // out and put back into the outputs of the rows that do
-          ok = mbar_wait_bounded(raw, raw_phase & 1, p.status, kAttnTimeout);
-          ++raw_phase;
-          if (ok) {
+      int raws = 0, it = 0, qs[2] = {0, 0};
+      TcWork w;
+      for (int k = 0; ok && item(k, w); ++k) {
+        const TcTiles t(p, w, tokens);
+        int* fx = fix + (k & 1) * kFixInts;
+        if (fixed[k & 1]) {  // the roles have left the item that used it last
+          for (int i = lane; i < kFixInts; i += 32) fx[i] = INT_MAX;
+          __syncwarp();
+          if (lane == 0) fixed[k & 1] = 0;
+          __syncwarp();
+        }
+        auto load_q = [&](int s) {
+          if (!t.n[s] || !ok) return;
+          ok = wait(q_empty + s, qs[s]++ + 1);
+          if (lane == 0 && ok) {
+            mbar_arrive_expect_tx(q_full + s, q_bytes);
             for (int h = 0; h < kHalves; ++h)
-              for (int r = max(0, min(seen, last)); r < kTcKeys; r += 4) {
-                const int row = r + (lane >> 3);
-                if (row < kTcKeys) {
-                  // 16-byte piece c of row r lies at piece c ^ (r % 8) (the 128-byte swizzle)
-                  uint4* at = reinterpret_cast<uint4*>(dst + h * 16384 + row * 128) + (lane & 7);
-                  if (row >= last) {
-                    *at = make_uint4(0, 0, 0, 0);
-                  } else {
-                    const uint4 x = *at;
-                    if (non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w)) {
-                      *at = take_non_finite<T>(x, j * kTcKeys + row, h * 64 + ((lane & 7) ^ (row & 7)) * 8, fix);
-                      *fixed = 1;
+              tma_load_4d(smem + L::kQ + s * L::kTile + h * 16384, &q_map, q_full + s, h * 64, 0, w.head, w.q0 + t.first[s]);
+          }
+        };
+        // one K or V tile; the bytes count whole boxes, what lies outside the tensor arrives as zeros
+        auto load_kv = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
+          if (lane == 0) mbar_arrive_expect_tx(bar, L::kTile);
+          __syncwarp();
+          if constexpr (kPaged) {
+            const int rows = min(1 << p.page_shift, kTcKeys);
+            const int key = j * kTcKeys + lane * rows;
+            if (lane * rows < kTcKeys) {
+              int page = p.kv_tokens;  // outside: zeros
+              if (key < t.key_end) {
+                const int id = __ldg(p.block_table + w.seq * p.table_stride + (key >> p.page_shift));
+                if (id >= 0 && id < p.kv_tokens) page = id; else atomicOr(p.status, kAttnBadPage);
+              }
+              for (int h = 0; h < kHalves; ++h)
+                tma_load_4d(dst + h * 16384 + lane * rows * 128, map, bar, h * 64, w.head, key & ((1 << p.page_shift) - 1), page);
+            }
+          } else if (lane == 0) {
+            for (int h = 0; h < kHalves; ++h) tma_load_3d(dst + h * 16384, map, bar, h * 64, w.head, w.k0 + j * kTcKeys);
+          }
+          __syncwarp();
+        };
+        load_q(0);
+        for (int i = 0; i < 2 * t.nmax && ok; ++i, ++it) {  // K0 K1 V0 K2 V1 ... as the products take them
+          const bool is_v = i + 1 == 2 * t.nmax || (i > 0 && !(i & 1));
+          const int slot = it % NS, j = is_v ? (i + 1 == 2 * t.nmax ? t.nmax : i >> 1) - 1 : (i + 1) >> 1;
+          uint8_t* dst = smem + L::kRing + slot * L::kTile;
+          ok = wait(kv_empty + slot, it / NS + 1);
+          if (!ok) break;
+          const int last = t.key_end - j * kTcKeys, seen = t.common - j * kTcKeys;  // rows of this tile below them
+          const bool clean = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
+          load_kv(is_v ? &v_map : &k_map, dst, clean ? raw : kv_full + slot, j);
+          if (i == 0) load_q(1);
+          if (clean) {
+            // P is 0 where a row does not see a key, but 0 * inf and 0 * NaN are not: rows behind the
+            // last key become zeros, and non-finite values of keys that only some rows see are taken
+            // out and put back into the outputs of the rows that do
+            ok = wait(raw, raws++) && ok;
+            if (ok) {
+              for (int h = 0; h < kHalves; ++h)
+                for (int r = max(0, min(seen, last)); r < kTcKeys; r += 4) {
+                  const int row = r + (lane >> 3);
+                  if (row < kTcKeys) {
+                    // 16-byte piece c of row r lies at piece c ^ (r % 8) (the 128-byte swizzle)
+                    uint4* at = reinterpret_cast<uint4*>(dst + h * 16384 + row * 128) + (lane & 7);
+                    if (row >= last) {
+                      *at = make_uint4(0, 0, 0, 0);
+                    } else {
+                      const uint4 x = *at;
+                      if (non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w)) {
+                        *at = take_non_finite<T>(x, j * kTcKeys + row, h * 64 + ((lane & 7) ^ (row & 7)) * 8, fx);
+                        fixed[k & 1] = 1;
+                      }
                     }
                   }
                 }
-              }
-            fence_proxy_async_smem();
+              fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(kv_full + slot);
           }
-          __syncwarp();
-          if (ok && lane == 0) mbar_arrive(kv_full + slot);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(w_empty + (k & 1));
       }
       if (!ok) {
         // a wait gave up: the loads in flight still have to land before the CTA may leave
@@ -264,81 +417,108 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mbar_wait_bounded(bar, i & 1, p.status, kAttnTimeout);
         }
       }
-      } else if (warp == 8) {
-      // ---------------------------------------------------------------- MMA issue
-      if (lane == 0 && nmax) {
-        const uint32_t id_s = tc_idesc<T>(kTcKeys, false), id_o = tc_idesc<T>((p.head_dim + 15) / 16 * 16, true);
-        const int steps = (p.head_dim + 15) / 16;
-        const uint32_t q_at = smem_u32(smem + L::kQ), ring = smem_u32(smem + L::kRing);
-        auto full = [&](int i) { return mbar_wait_bounded(kv_full + i % NS, (i / NS) & 1, p.status, kAttnTimeout); };
-        auto scores = [&](int s, int i) {  // S_s = Q_s K^T, K in ring item i
-          const uint32_t a = q_at + s * L::kTile, b = ring + (i % NS) * L::kTile;
-          for (int k = 0; k < steps; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            tc_mma<true>(tmem + s * 128, desc_sw128(a + off, 16, 1024), desc_sw128(b + off, 16, 1024), id_s, k != 0);
-          }
-          tc_commit(s_full + s);
-        };
-        bool ok = mbar_wait_bounded(q_full, 0, p.status, kAttnTimeout) && full(0);
-        if (ok) {
-          tc_fence_after();
-          if (n[0]) scores(0, 0);
-          if (n[1]) {
-            ok = mbar_wait_bounded(q_full + 1, 0, p.status, kAttnTimeout);
-            if (ok) scores(1, 0);
-          }
-          tc_commit(kv_empty);
-        }
-        for (int j = 0; j < nmax && ok; ++j) {
-          const int iv = 2 * j + 1, ik = 2 * j + 2;
-          ok = full(iv) && (j + 1 == nmax || full(ik));
-          for (int s = 0; s < 2 && ok; ++s) {
-            if (j >= n[s]) continue;
-            ok = mbar_wait_bounded(p_full + s, j & 1, p.status, kAttnTimeout);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t b = ring + (iv % NS) * L::kTile;
-#pragma unroll
-            for (int k = 0; k < kTcKeys / 16; ++k)
-              tc_mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, desc_sw128(b + k * 2048, 16384, 1024), id_o, (j | k) != 0);
-            tc_commit(o_done + s);
-            if (j + 1 < n[s]) scores(s, ik);
-          }
-          if (ok) {
-            tc_commit(kv_empty + iv % NS);
-            if (j + 1 < nmax) tc_commit(kv_empty + ik % NS);
-          }
-        }
-        if (!ok) {  // a wait gave up: the products in flight end before TMEM is freed
-          tc_commit(drain);
-          mbar_wait_bounded(drain, 0, p.status, kAttnTimeout);
-        }
-      }
-      __syncwarp();
-      }
-    } else {
-      // ---------------------------------------------------------------- softmax: one row per thread
-      regs_up<216>();
-      const int s = warp >> 2, row = threadIdx.x & 127;
-      const int token = first[s] + row / p.group;
-      const bool mine = row < tokens * p.group && row / p.group < valid[s];
-      const int seen = mine ? keys_seen(token, w.len_q, w.len_k, p.causal) : 0;
-      const int all_see = valid[s] ? keys_seen(first[s], w.len_q, w.len_k, p.causal) : 0;
-      const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 TMEM lanes
-      const uint32_t s_at = lanes + s * 128, o_at = lanes + 256 + s * 128;
-      const float scale = fmaxf(p.scale, 1e-30f);  // 0 would make NaN of a masked score's -inf
-      const float sl2 = scale * 1.4426950408889634f;
-      float m = -INFINITY, l = 0.f;
+    } else if (lane == 0) {
+      // ---------------------------------------------------------------- MMA issue, one thread per row tile
+      const int s = warp == 8 ? 0 : 1;
+      const uint32_t id_s = tc_idesc<T>(kTcKeys, false), id_o = tc_idesc<T>((p.head_dim + 15) / 16 * 16, true);
+      const int steps = (p.head_dim + 15) / 16;
+      // descriptors of the first K step; later steps and slots add to the address field
+      const uint64_t q_desc = desc_sw128(smem_u32(smem + L::kQ + s * L::kTile), 16, 1024);
+      const uint64_t k_desc = desc_sw128(smem_u32(smem + L::kRing), 16, 1024);
+      const uint64_t v_desc = desc_sw128(smem_u32(smem + L::kRing), 16384, 1024);
+      const uint32_t p_at = tmem + 128 + s * 64, o_at = tmem + 256 + s * 128;
       bool ok = true;
-      for (int j = 0; j < n[s]; ++j) {
-        ok = mbar_wait_bounded(s_full + s, j & 1, p.status, kAttnTimeout);
-        ok = __all_sync(~0u, ok);
+      int it = 0, qs = 0, ps = 0;
+      auto full = [&](int i) { return wait(kv_full + i % NS, i / NS); };
+      TcWork w;
+      for (int k = 0; ok && item(k, w); ++k) {
+        const TcTiles t(p, w, tokens);
+        const int n = s ? t.n[1] : t.n[0];
+        // every ring item in order, K0 K1 V0 K2 V1 ..., also those that only the other tile uses
+        for (int j = -1; j < t.nmax && ok; ++j) {
+          if (j + 1 < t.nmax) {  // S = Q K^T for key tile j + 1
+            const int i = it + (j < 0 ? 0 : 2 * j + 1);
+            ok = full(i);
+            if (j < 0 && n && ok) ok = wait(q_full + s, qs++);
+            // S's place goes tile 0, tile 1, tile 0 ...: it is this tile's once the other's scores have left it.  A
+            // tile without this key tile passes its turn on, so that both count the same phases.
+            const int turn = (it >> 1) + j + 1;
+            if (ok && (s || turn)) ok = s ? wait(s_free, turn) : wait(s_free + 1, turn - 1);
+            if (!ok) break;
+            if (j + 1 < n) {
+              tc_fence_after();
+              const uint64_t b = k_desc + (i % NS) * (L::kTile >> 4);
+#pragma unroll
+              for (int c = 0; c < DP / 16; ++c) {
+                const int off = ((c >> 2) * 16384 + (c & 3) * 32) >> 4;
+                if (c < steps) tc_mma<true>(tmem, q_desc + off, b + off, id_s, c != 0);
+              }
+              tc_commit(s_full + s);
+              tc_commit(kv_empty + i % NS);
+              if (j + 2 == n) tc_commit(q_empty + s);  // the tile's last score product
+            } else {
+              mbar_arrive_count(s_free + s, 128);
+              mbar_arrive(kv_empty + i % NS);
+            }
+          }
+          if (j >= 0 && ok) {  // O += P V for key tile j
+            const int i = it + (j + 1 < t.nmax ? 2 * j + 2 : 2 * t.nmax - 1);
+            ok = full(i);
+            if (j < n) {
+              ok = ok && wait(p_full + s, ps++);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t b = v_desc + (i % NS) * (L::kTile >> 4);
+#pragma unroll
+              for (int c = 0; c < kTcKeys / 16; ++c)
+                tc_mma_ts(o_at, p_at + c * 8, b + c * (2048 >> 4), id_o, (j | c) != 0);
+              tc_commit(o_done + s);
+              tc_commit(kv_empty + i % NS);
+            } else if (ok) {
+              mbar_arrive(kv_empty + i % NS);
+            }
+          }
+        }
+        if (!ok) break;
+        it += 2 * t.nmax;
+        mbar_arrive(w_empty + (k & 1));
+      }
+      if (!ok) {  // a wait gave up: the products in flight end before TMEM is freed
+        tc_commit(drain + s);
+        mbar_wait_bounded(drain + s, 0, p.status, kAttnTimeout);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax: one row per thread
+    regs_up<216>();
+    const int s = warp >> 2, row = threadIdx.x & 127;
+    const int row_token = row / p.group, row_head = row % p.group;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 TMEM lanes
+    const uint32_t p_at = lanes + 128 + s * 64, o_at = lanes + 256 + s * 128;
+    const float scale = fmaxf(p.scale, 1e-30f);  // 0 would make NaN of a masked score's -inf
+    const float sl2 = scale * 1.4426950408889634f;
+    bool ok = true;
+    int done = 0;  // key tiles of this row tile so far, over all items
+    TcWork w;
+    for (int k = 0; ok && __all_sync(~0u, item(k, w)); ++k) {
+      const TcTiles t(p, w, tokens);
+      const int first = s ? t.first[1] : t.first[0], valid = s ? t.valid[1] : t.valid[0], n = s ? t.n[1] : t.n[0];
+      const int token = first + row_token;
+      const bool mine = row_token < valid;  // rows behind the last whole token have row_token >= tokens
+      const int seen = mine ? keys_seen(token, w.len_q, w.len_k, p.causal) : 0;
+      const int all_see = valid ? keys_seen(first, w.len_q, w.len_k, p.causal) : 0;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++done) {
+        ok = __all_sync(~0u, wait(s_full + s, done));
         if (!ok) break;
         tc_fence_after();
         uint32_t x[128];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(lanes + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
         tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(s_free + s);
         if ((j + 1) * kTcKeys > all_see) {
           const int lim = seen - j * kTcKeys;
 #pragma unroll
@@ -347,10 +527,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 128; c += 4)
+        for (int c = 0; c < 128; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(x[c + e]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
+        const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
         const bool move = (top - m) * sl2 > kLazyLog2;  // from -inf too
         if (__any_sync(~0u, move)) {
           const float old = m;
@@ -358,17 +538,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const float f = move ? exp2_sfu((old - m) * sl2) : 1.f;
           l *= f;
           if (__any_sync(~0u, move && old != -INFINITY)) {
-            ok = mbar_wait_bounded(o_done + s, (j - 1) & 1, p.status, kAttnTimeout);
-            ok = __all_sync(~0u, ok);
+            ok = __all_sync(~0u, wait(o_done + s, done - 1));
             if (!ok) break;
             tc_fence_after();
-            uint32_t o[32];
-            for (int c = 0; c < DP; c += 32) {
-              tmem_ld_32x32(o_at + c, o);
+            uint32_t o[16];
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 16) {
+              tmem_ld_32x16(o_at + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st_32x32(o_at + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st_32x16(o_at + c, o);
             }
             tmem_st_wait();
           }
@@ -385,8 +565,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
           x[c >> 1] = pack16<T>(a, b);
         }
-        tmem_st_32x32(s_at, x);
-        tmem_st_32x32(s_at + 32, x + 32);
+        if (j > 0) {  // the last P has been consumed
+          ok = __all_sync(~0u, wait(o_done + s, done - 1));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        tmem_st_32x32(p_at, x);
+        tmem_st_32x32(p_at + 32, x + 32);
         float a, b;
         f2_unpack(f2_add(sum[0], sum[1]), a, b);
         l += a + b;
@@ -394,18 +579,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
         mbar_arrive(p_full + s);
       }
-      if (ok && n[s]) ok = mbar_wait_bounded(o_done + s, (n[s] - 1) & 1, p.status, kAttnTimeout);
-      ok = __all_sync(~0u, ok);
-      if (ok && valid[s]) {
+      if (ok && n) ok = __all_sync(~0u, wait(o_done + s, done - 1));
+      if (ok && valid) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t tok = w.q0 + token;
-        const int qh = head * p.group + row % p.group;
+        const int qh = w.head * p.group + row_head;
         T* dst = static_cast<T*>(p.out) + tok * p.o_ts + qh * p.o_hs;
-        const bool patch = *reinterpret_cast<volatile int*>(fixed) != 0;
+        const bool patch = *reinterpret_cast<volatile int*>(fixed + (k & 1)) != 0;
+        const int* fx = fix + (k & 1) * kFixInts;
         for (int c = 0; c < p.head_dim; c += 32) {
           uint32_t o[32];
-          if (n[s]) {
+          if (n) {
             tmem_ld_32x32(o_at + c, o);
             tmem_ld_wait();
           } else {
@@ -423,8 +608,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 float a = __uint_as_float(o[i]) * inv, b = __uint_as_float(o[i + 1]) * inv;
                 if (seen == 0) a = b = 0.f;
                 if (patch) {
-                  a = put_back(a, fix, c + i, seen);
-                  b = put_back(b, fix, c + i + 1, seen);
+                  a = put_back(a, fx, c + i, seen);
+                  b = put_back(b, fx, c + i + 1, seen);
                 }
                 y[e] = pack16<T>(a, b);
               }
@@ -433,7 +618,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         if (mine && p.lse) p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, scale, logf(l));
+        tc_fence_before();  // these reads of O before the next item's first product into it
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(w_empty + (k & 1));
     }
   }
   tc_fence_before();

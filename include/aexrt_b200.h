@@ -480,7 +480,8 @@ typedef struct AexrtB200AttentionDesc {
     float scale;          /* finite, >= 0 */
     uint32_t kv_tokens;   /* packed: rows of k and v.  paged: pages of the cache */
     uint32_t page_size;   /* paged: tokens per page, a power of two from 8 to 1024 */
-    uint32_t table_columns, table_stride; /* paged: columns of block_table, elements between its rows */
+    uint32_t table_columns, table_stride; /* paged: columns of block_table (times page_size at most 2^30), elements
+                                             between its rows */
     uint64_t q_token_stride, q_head_stride;
     uint64_t out_token_stride, out_head_stride;
     uint64_t k_token_stride, k_head_stride, k_page_stride; /* page strides: paged only */

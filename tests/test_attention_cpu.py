@@ -63,6 +63,7 @@ def test_attention_descriptions_are_refused(kw, msg):
 @pytest.mark.parametrize("kw,msg", [
     (dict(page_size=0), "page_size"), (dict(page_size=4), "page_size"), (dict(page_size=24), "page_size"),
     (dict(page_size=2048), "page_size"), (dict(table_stride=3), "table_stride"), (dict(k_page_stride=12), "multiples of 8"),
+    (dict(table_columns=(1 << 26) + 1, table_stride=1 << 27), "2^30 tokens"),
 ])
 def test_paged_descriptions_are_refused(kw, msg):
     lib = _native.load()

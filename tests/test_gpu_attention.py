@@ -200,6 +200,29 @@ def test_packed_visible_non_finite_values_come_through(bad):
         oracle.check(out, lse, *want)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_non_finite_score_makes_its_rows_nan(bad, dtype):
+    """A visible key with NaN, or whose score overflows to +inf, wherever in a tile it lies; other rows are left alone."""
+    g = generator(32)
+    n, d = 300, 64
+    q = rand(g, n, 1, d, dtype=dtype).abs() + 0.1  # every score with an infinite key is +inf
+    k, v = (rand(g, n, 1, d, dtype=dtype) for _ in range(2))
+    cu, page = ints([0, n]), 16
+    clean = ops.attention_packed(q, k, v, cu, cu)
+    table = torch.arange(-(-n // page), dtype=torch.int32, device="cuda")[None]
+    for key in list(range(0, n, 7)) + [0, 31, 32, 127, 128, n - 1]:
+        kk = k.clone()
+        kk[key] = bad
+        out, lse = ops.attention_packed(q, kk, v, cu, cu, return_lse=True)
+        assert torch.equal(out[:key], clean[:key])
+        assert bool(torch.isnan(out[key:]).all()) and bool(torch.isnan(lse[key:]).all())
+        kc, vc = (torch.zeros(table.shape[1], page, 1, d, dtype=dtype, device="cuda") for _ in range(2))
+        ops.kv_append(kk, v, torch.arange(n, dtype=torch.int32, device="cuda"), kc, vc)
+        out = ops.attention_paged(q[-3:], kc, vc, table, ints([0, 3]), ints([n]), 3)
+        assert bool(torch.isnan(out[-1]).all()) and (key > n - 3 or bool(torch.isnan(out).all()))
+
+
 def test_packed_large_and_rising_scores():
     """Scores that grow along the keys, so that the running maximum keeps moving, and scores far below it."""
     for dtype in (F16, BF16):
@@ -237,6 +260,24 @@ def test_packed_many_short_sequences():
     no_status()
     want = expect(q, split(k, lens), split(v, lens), lens, 32 ** -0.5, True)
     oracle.check(out[:sum(lens)], lse[:sum(lens)], *want)
+
+
+@pytest.mark.parametrize("n", [100, 128, 129, 300])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_every_item_is_taken_once(n, causal):
+    """Many sequences of very different lengths: the order of the work (by keys, or by sequence when there are many) leaves
+    nothing out; rows nobody writes would keep the sentinel."""
+    rng = random.Random(n)
+    q_lens = [rng.choice([0, 1, 3, 130, 257, rng.randint(1, 500)]) for _ in range(n)]
+    k_lens = [rng.choice([x, x, 0, rng.randint(0, 700)]) for x in q_lens]
+    g = generator(n)
+    q = rand(g, sum(q_lens), 4, 64, dtype=BF16)
+    k, v = (rand(g, sum(k_lens), 2, 64, dtype=BF16) for _ in range(2))
+    out = torch.full_like(q, 1000.0)
+    out, lse = ops.attention_packed(q, k, v, ints(oracle.sums(q_lens)), ints(oracle.sums(k_lens)), causal=causal, out=out,
+                                    return_lse=True)
+    no_status()
+    oracle.check(out, lse, *expect(q, split(k, k_lens), split(v, k_lens), q_lens, 0.125, causal))
 
 
 def test_packed_long_sequence():
