@@ -20,7 +20,8 @@
 //
 // One CTA per SM stays for all its items: the loads, the score products and the search of the next
 // item go on while the softmax warps write the last one's output.  Items go out in the order of their key tiles,
-// the longest first, so that ragged batches and the causal triangle end evenly.
+// the longest first, one to each CTA in turn and every other turn backwards, so that ragged batches
+// and the causal triangle end evenly.
 //
 // Roles: warps 0-3 softmax of tile 0, warps 4-7 of tile 1, one thread each of warps 8 and 11 issues
 // the MMAs of tile 0 and of tile 1 (one thread for both spent 93 clocks an MMA instead of the
@@ -131,21 +132,30 @@ struct TcFinder {
     }
   }
   __device__ __forceinline__ int rows_of(int s) const { return kPaged ? min(q_len(p, s), p.max_q) : q_len(p, s); }
-  // Items of held sequence h of this lane with at least `level` key tiles.
+  // Items of held sequence h of this lane with at least `level` key tiles, its last item aside.
   __device__ __forceinline__ int items_from(int h, int level) const {
-    const int all = (rows[h] + tokens - 1) / tokens;
-    if (level <= 0) return all;
+    const int before_last = max(0, (rows[h] + tokens - 1) / tokens - 1);
+    if (level <= 0) return before_last;
     if (level > tiles[h]) return 0;
-    if (!p.causal) return all;
-    // item t ends at token e = min((t + 1) * tokens, rows) and sees e + shift keys
+    if (!p.causal) return before_last;
+    // item t ends at token e = (t + 1) * tokens and sees e + shift keys
     const int e = (level - 1) * kTcKeys + 1 - shift[h];
-    return e <= 0 ? all : all - (e + tokens - 1) / tokens + 1;
+    return e <= 0 ? before_last : max(0, before_last - (e + tokens - 1) / tokens + 1);
+  }
+  // The last item counts half its key tiles when it fills one row tile only.
+  __device__ __forceinline__ int last_level(int h) const {
+    const int all = (rows[h] + tokens - 1) / tokens;
+    if (all == 0) return -1;
+    return rows[h] - (all - 1) * tokens <= tokens / 2 ? (tiles[h] + 1) / 2 : tiles[h];
+  }
+  __device__ __forceinline__ int all_items_from(int h, int level) const {
+    return items_from(h, level) + (last_level(h) >= max(level, 0) ? 1 : 0);
   }
   __device__ __forceinline__ int64_t all_from(int level) const {
     int64_t n = 0;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
-      if (32 * h < p.num_seqs) n += items_from(h, level);
+      if (32 * h < p.num_seqs) n += all_items_from(h, level);
 #pragma unroll
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
     return n;
@@ -176,7 +186,8 @@ struct TcFinder {
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
         if (32 * h >= p.num_seqs) break;
-        const int above = items_from(h, lo + 1), n = items_from(h, lo) - above;
+        const int above = items_from(h, lo + 1), here = items_from(h, lo) - above;
+        const int n = here + (last_level(h) == lo ? 1 : 0);
         int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -186,9 +197,9 @@ struct TcFinder {
         const uint32_t past = __ballot_sync(~0u, sum > rank);
         if (past) {
           const int src = __ffs(past) - 1;
-          const int all = (rows[h] + tokens - 1) / tokens;
-          // a sequence's later items see more keys: those above this level are its last ones
-          const int tile = all - 1 - above - static_cast<int>(rank - (sum - n));
+          const int all = (rows[h] + tokens - 1) / tokens, off = static_cast<int>(rank - (sum - n));
+          // a sequence's later items see more keys: those above this level are the last ones before its last item
+          const int tile = off < here ? all - 2 - above - off : all - 1;
           fill(w, 32 * h + src, __shfl_sync(~0u, tile, src));
           return true;
         }
@@ -311,7 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // ---------------------------------------------------------------- items
       TcFinder<kPaged> finder(p, 2 * tokens);
       for (int k = 0;; ++k) {
-        const int64_t number = static_cast<int64_t>(k) * gridDim.x + blockIdx.x;
+        const int64_t number = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         TcWork w = {};
         const bool found = finder.find(number / p.kv_heads, w);
         w.head = found ? static_cast<int>(number % p.kv_heads) : -1;
@@ -327,19 +338,77 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t q_bytes = static_cast<uint32_t>(tokens * p.group * 128 * kHalves);
       bool ok = true;
       int raws = 0, it = 0, qs[2] = {0, 0};
+      // A V tile that has to be cleaned before its product.  P is 0 where a row does not see a key, but
+      // 0 * inf and 0 * NaN are not: rows behind the last key become zeros, and non-finite values of
+      // keys that only some rows see are taken out and put back into the outputs of the rows that do.
+      // The tile lands on a barrier of its own and is cleaned while later loads are already on their way.
+      bool dirty = false;
+      int d_slot = 0, d_item = 0, d_from = 0, d_last = 0, d_key = 0;  // rows from .. last are looked at
+      bool d_release = false;  // the item has no other loads left
+      auto clean = [&]() {
+        uint8_t* dst = smem + L::kRing + d_slot * L::kTile;
+        int* fx = fix + (d_item & 1) * kFixInts;
+        const int sub = lane >> 3, piece = lane & 7;  // 16-byte piece c of row r lies at piece c ^ (r % 8): the 128-byte swizzle
+        for (int h = 0; h < kHalves; ++h) {
+          uint4* tile = reinterpret_cast<uint4*>(dst + h * 16384) + piece;
+#pragma unroll 4
+          for (int r = d_last + sub; r < kTcKeys; r += 4) tile[r * 8] = make_uint4(0, 0, 0, 0);
+          for (int r = d_from + sub; r < d_last; r += 32) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {  // rows past the end look at this lane's first row again
+              const uint4 x = tile[(r + 4 * u < d_last ? r + 4 * u : r) * 8];
+              bits |= non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w);
+            }
+            if (bits) {
+              for (int row = r; row < min(r + 32, d_last); row += 4)
+                tile[row * 8] = take_non_finite<T>(tile[row * 8], d_key + row, h * 64 + (piece ^ (row & 7)) * 8, fx);
+              fixed[d_item & 1] = 1;
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(kv_full + d_slot);
+          if (d_release) mbar_arrive(w_empty + (d_item & 1));
+        }
+        dirty = d_release = false;
+      };
+      auto flush = [&]() {  // the tile to be cleaned, now
+        if (dirty && ok) {
+          ok = __all_sync(~0u, wait(raw, raws++));
+          if (ok) clean();
+        }
+      };
+      auto wait_serving = [&](uint64_t* bar, int phase) {  // a wait that cleans the tile when that lands first
+        const long long t0 = clock64();
+        while (dirty) {
+          if (__any_sync(~0u, mbar_test_wait(bar, phase & 1))) return true;
+          if (__any_sync(~0u, mbar_test_wait(raw, raws & 1))) {
+            ++raws;
+            clean();
+          } else if (__any_sync(~0u, clock64() - t0 > kWaitLimitCycles)) {
+            break;
+          }
+        }
+        return __all_sync(~0u, wait(bar, phase)) != 0;
+      };
       TcWork w;
-      for (int k = 0; ok && item(k, w); ++k) {
+      for (int k = 0; ok; ++k) {
+        ok = wait_serving(w_full + (k & 1), k >> 1);
+        w = work[k & 1];
+        if (!ok || w.head < 0) break;
         const TcTiles t(p, w, tokens);
-        int* fx = fix + (k & 1) * kFixInts;
         if (fixed[k & 1]) {  // the roles have left the item that used it last
-          for (int i = lane; i < kFixInts; i += 32) fx[i] = INT_MAX;
           __syncwarp();
+          for (int i = lane; i < kFixInts; i += 32) fix[(k & 1) * kFixInts + i] = INT_MAX;
           if (lane == 0) fixed[k & 1] = 0;
           __syncwarp();
         }
         auto load_q = [&](int s) {
           if (!t.n[s] || !ok) return;
-          ok = wait(q_empty + s, qs[s]++ + 1);
+          ok = wait_serving(q_empty + s, qs[s]++ + 1);
           if (lane == 0 && ok) {
             mbar_arrive_expect_tx(q_full + s, q_bytes);
             for (int h = 0; h < kHalves; ++h)
@@ -371,45 +440,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < 2 * t.nmax && ok; ++i, ++it) {  // K0 K1 V0 K2 V1 ... as the products take them
           const bool is_v = i + 1 == 2 * t.nmax || (i > 0 && !(i & 1));
           const int slot = it % NS, j = is_v ? (i + 1 == 2 * t.nmax ? t.nmax : i >> 1) - 1 : (i + 1) >> 1;
-          uint8_t* dst = smem + L::kRing + slot * L::kTile;
-          ok = wait(kv_empty + slot, it / NS + 1);
-          if (!ok) break;
           const int last = t.key_end - j * kTcKeys, seen = t.common - j * kTcKeys;  // rows of this tile below them
-          const bool clean = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
-          load_kv(is_v ? &v_map : &k_map, dst, clean ? raw : kv_full + slot, j);
+          const bool unclean = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
+          if (unclean) flush();
+          ok = ok && wait_serving(kv_empty + slot, it / NS + 1);
+          if (!ok) break;
+          load_kv(is_v ? &v_map : &k_map, smem + L::kRing + slot * L::kTile, unclean ? raw : kv_full + slot, j);
           if (i == 0) load_q(1);
-          if (clean) {
-            // P is 0 where a row does not see a key, but 0 * inf and 0 * NaN are not: rows behind the
-            // last key become zeros, and non-finite values of keys that only some rows see are taken
-            // out and put back into the outputs of the rows that do
-            ok = wait(raw, raws++) && ok;
-            if (ok) {
-              for (int h = 0; h < kHalves; ++h)
-                for (int r = max(0, min(seen, last)); r < kTcKeys; r += 4) {
-                  const int row = r + (lane >> 3);
-                  if (row < kTcKeys) {
-                    // 16-byte piece c of row r lies at piece c ^ (r % 8) (the 128-byte swizzle)
-                    uint4* at = reinterpret_cast<uint4*>(dst + h * 16384 + row * 128) + (lane & 7);
-                    if (row >= last) {
-                      *at = make_uint4(0, 0, 0, 0);
-                    } else {
-                      const uint4 x = *at;
-                      if (non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w)) {
-                        *at = take_non_finite<T>(x, j * kTcKeys + row, h * 64 + ((lane & 7) ^ (row & 7)) * 8, fx);
-                        fixed[k & 1] = 1;
-                      }
-                    }
-                  }
-                }
-              fence_proxy_async_smem();
-            }
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(kv_full + slot);
+          if (unclean) {
+            dirty = true;
+            d_slot = slot;
+            d_item = k;
+            d_last = min(last, kTcKeys);
+            d_from = max(0, min(seen, d_last));
+            d_key = j * kTcKeys;
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(w_empty + (k & 1));
+        if (dirty && d_item == k) d_release = true;
+        else if (lane == 0) mbar_arrive(w_empty + (k & 1));
       }
+      flush();
       if (!ok) {
         // a wait gave up: the loads in flight still have to land before the CTA may leave
         for (int i = 0; i < 2 * (NS + 3); ++i) {
