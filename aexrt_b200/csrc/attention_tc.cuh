@@ -40,14 +40,15 @@ constexpr int kTcRows = 128;   // query rows of a tile
 constexpr int kTcKeys = 128;   // keys of a tile
 constexpr int kTcThreads = 384;
 
-// Slots of the K / V ring (K and V tiles alternate): what 227 KB hold beside the two Q tiles.
+// Slots of the K / V ring: what 227 KB hold beside the two Q tiles and the output staging.
 template <int DP>
-constexpr int tc_slots() { return DP == 128 ? 5 : 8; }
+constexpr int tc_slots() { return DP == 128 ? 4 : 8; }
 
 template <int DP>
 struct TcSmem {
   static constexpr int kTile = 128 * DP * 2;
-  static constexpr int kQ = 0, kRing = 2 * kTile, kBars = kRing + tc_slots<DP>() * kTile;
+  static constexpr int kQ = 0, kRing = 2 * kTile, kStage = kRing + tc_slots<DP>() * kTile;
+  static constexpr int kBars = kStage + 8 * 4096;  // per softmax warp: 32 rows of 64 output columns
   // barriers, TMEM base, items; then, per item of two, the first keys with non-finite values of a column
   static constexpr int kFix = kBars + 512, kBytes = kFix + 2 * kFixInts * 4;
 };
@@ -111,54 +112,60 @@ template <bool kPaged>
 struct TcFinder {
   static constexpr int kHeld = 4;
   const AttnParams& p;
-  int tokens;  // query tokens of an item
-  int rows[kHeld], shift[kHeld], tiles[kHeld];  // of sequence 32 * h + lane: rows, len_k - len_q, key tiles of the last item
-  int base = 0;      // by sequence: the first sequence of the 32 looked at, and the items before it
+  int tokens;      // query tokens of an item
+  float per_token; // 1 / tokens
+  // of sequence 32 * h + lane: items, len_k - len_q, key tiles of the last item and what that counts for
+  int items[kHeld], shift[kHeld], tiles[kHeld], last[kHeld];
+  int total = 0, top = 0;  // of all sequences: items, key tiles at most
+  int base = 0;            // by sequence: the first sequence of the 32 looked at, and the items before it
   int64_t before = 0;
 
   __device__ __forceinline__ TcFinder(const AttnParams& params, int tokens_) : p(params), tokens(tokens_) {
+    per_token = 1.f / static_cast<float>(tokens);
     if (p.num_seqs <= 32 * kHeld) {
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
         const int s = 32 * h + (threadIdx.x & 31);
-        rows[h] = shift[h] = tiles[h] = 0;
+        items[h] = shift[h] = tiles[h] = 0;
+        last[h] = -1;
         if (s < p.num_seqs) {
-          const int len_k = k_len<kPaged>(p, s);
-          rows[h] = rows_of(s);
-          shift[h] = len_k - q_len(p, s);
-          tiles[h] = rows[h] ? (keys_seen(rows[h] - 1, q_len(p, s), len_k, p.causal) + kTcKeys - 1) / kTcKeys : 0;
+          const int len_q = q_len(p, s), len_k = k_len<kPaged>(p, s), rows = kPaged ? min(len_q, p.max_q) : len_q;
+          items[h] = (rows + tokens - 1) / tokens;
+          shift[h] = len_k - len_q;
+          if (rows) {
+            tiles[h] = (keys_seen(rows - 1, len_q, len_k, p.causal) + kTcKeys - 1) / kTcKeys;
+            // the last item counts half its key tiles when it fills one row tile only
+            last[h] = rows - (items[h] - 1) * tokens <= tokens / 2 ? (tiles[h] + 1) / 2 : tiles[h];
+          }
         }
+        total += items[h];
+        top = max(top, tiles[h]);
       }
+      total = __reduce_add_sync(~0u, total);
+      top = __reduce_max_sync(~0u, top);
     }
   }
   __device__ __forceinline__ int rows_of(int s) const { return kPaged ? min(q_len(p, s), p.max_q) : q_len(p, s); }
   // Items of held sequence h of this lane with at least `level` key tiles, its last item aside.
   __device__ __forceinline__ int items_from(int h, int level) const {
-    const int before_last = max(0, (rows[h] + tokens - 1) / tokens - 1);
+    const int before_last = max(0, items[h] - 1);
     if (level <= 0) return before_last;
     if (level > tiles[h]) return 0;
     if (!p.causal) return before_last;
-    // item t ends at token e = (t + 1) * tokens and sees e + shift keys
+    // item t ends at token e = (t + 1) * tokens and sees e + shift keys: the first ceil(e / tokens) - 1 see too few
     const int e = (level - 1) * kTcKeys + 1 - shift[h];
-    return e <= 0 ? before_last : max(0, before_last - (e + tokens - 1) / tokens + 1);
+    if (e <= 0) return before_last;
+    int few = static_cast<int>(static_cast<float>(e - 1) * per_token);  // floor((e - 1) / tokens), then made exact
+    while (few * static_cast<int64_t>(tokens) > e - 1) --few;
+    while ((few + 1) * static_cast<int64_t>(tokens) <= e - 1) ++few;
+    return max(0, before_last - few);
   }
-  // The last item counts half its key tiles when it fills one row tile only.
-  __device__ __forceinline__ int last_level(int h) const {
-    const int all = (rows[h] + tokens - 1) / tokens;
-    if (all == 0) return -1;
-    return rows[h] - (all - 1) * tokens <= tokens / 2 ? (tiles[h] + 1) / 2 : tiles[h];
-  }
-  __device__ __forceinline__ int all_items_from(int h, int level) const {
-    return items_from(h, level) + (last_level(h) >= max(level, 0) ? 1 : 0);
-  }
-  __device__ __forceinline__ int64_t all_from(int level) const {
-    int64_t n = 0;
+  __device__ __forceinline__ int all_from(int level) const {
+    int n = 0;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
-      if (32 * h < p.num_seqs) n += all_items_from(h, level);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
-    return n;
+      if (32 * h < p.num_seqs) n += items_from(h, level) + (last[h] >= max(level, 0) ? 1 : 0);
+    return __reduce_add_sync(~0u, n);
   }
   __device__ __forceinline__ void fill(TcWork& w, int s, int tile) const {
     w.seq = s;
@@ -172,22 +179,18 @@ struct TcFinder {
   __device__ __forceinline__ bool find(int64_t item, TcWork& w) {
     const int lane = threadIdx.x & 31;
     if (p.num_seqs <= 32 * kHeld) {
-      if (item >= all_from(0)) return false;
-      int lo = 0, hi = 0;  // the highest level that has more than `item` items at or above it
-#pragma unroll
-      for (int h = 0; h < kHeld; ++h) hi = max(hi, tiles[h]);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) hi = max(hi, __shfl_xor_sync(~0u, hi, o));
+      if (item >= total) return false;
+      int lo = 0, hi = top;  // the highest level that has more than `item` items at or above it
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (all_from(mid) > item) lo = mid; else hi = mid - 1;
       }
-      int64_t rank = item - all_from(lo + 1);  // among the items of exactly this level
+      int rank = static_cast<int>(item) - all_from(lo + 1);  // among the items of exactly this level
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
         if (32 * h >= p.num_seqs) break;
         const int above = items_from(h, lo + 1), here = items_from(h, lo) - above;
-        const int n = here + (last_level(h) == lo ? 1 : 0);
+        const int n = here + (last[h] == lo ? 1 : 0);
         int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -197,9 +200,9 @@ struct TcFinder {
         const uint32_t past = __ballot_sync(~0u, sum > rank);
         if (past) {
           const int src = __ffs(past) - 1;
-          const int all = (rows[h] + tokens - 1) / tokens, off = static_cast<int>(rank - (sum - n));
+          const int off = rank - (sum - n);
           // a sequence's later items see more keys: those above this level are the last ones before its last item
-          const int tile = off < here ? all - 2 - above - off : all - 1;
+          const int tile = off < here ? items[h] - 2 - above - off : items[h] - 1;
           fill(w, 32 * h + src, __shfl_sync(~0u, tile, src));
           return true;
         }
@@ -636,37 +639,59 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t tok = w.q0 + token;
         const int qh = w.head * p.group + row_head;
-        T* dst = static_cast<T*>(p.out) + tok * p.o_ts + qh * p.o_hs;
+        const uint64_t dst = reinterpret_cast<uint64_t>(static_cast<T*>(p.out) + tok * p.o_ts + qh * p.o_hs);
+        const uint32_t owned = __ballot_sync(~0u, mine);
         const bool patch = *reinterpret_cast<volatile int*>(fixed + (k & 1)) != 0;
         const int* fx = fix + (k & 1) * kFixInts;
-        for (int c = 0; c < p.head_dim; c += 32) {
-          uint32_t o[32];
-          if (n) {
-            tmem_ld_32x32(o_at + c, o);
-            tmem_ld_wait();
-          } else {
+        // 64 columns at a time through shared memory (16-byte piece c of row r at c ^ (r % 8)): a store
+        // instruction then writes whole 128-byte lines of four rows instead of 16 bytes of 32
+        uint8_t* stage = smem + L::kStage + warp * 4096;
+        for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
+          for (int c = c0; c < min(c0 + 64, p.head_dim); c += 32) {
+            uint32_t o[32];
+            if (n) {
+              tmem_ld_32x32(o_at + c, o);
+              tmem_ld_wait();
+            } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0;
-          }
-          if (mine) {
+              for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if (seen == 0) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if (patch) {
+#pragma unroll 1
+              for (int e = 0; e < 32; ++e) {
+                // a loop over registers by number: every value moves up by one place
+                const float y = put_back(__uint_as_float(o[0]) * inv, fx, c + e, seen);
+#pragma unroll
+                for (int i = 0; i < 31; ++i) o[i] = o[i + 1];
+                o[31] = __float_as_uint(y);
+              }
+            }
+            const float f = patch ? 1.f : inv;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-              if (c + 8 * v >= p.head_dim) break;
               uint32_t y[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int i = 8 * v + 2 * e;
-                float a = __uint_as_float(o[i]) * inv, b = __uint_as_float(o[i + 1]) * inv;
-                if (seen == 0) a = b = 0.f;
-                if (patch) {
-                  a = put_back(a, fx, c + i, seen);
-                  b = put_back(b, fx, c + i + 1, seen);
-                }
-                y[e] = pack16<T>(a, b);
-              }
-              *reinterpret_cast<uint4*>(dst + c + 8 * v) = make_uint4(y[0], y[1], y[2], y[3]);
+              for (int e = 0; e < 4; ++e)
+                y[e] = pack16<T>(__uint_as_float(o[8 * v + 2 * e]) * f, __uint_as_float(o[8 * v + 2 * e + 1]) * f);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c - c0) / 8 + v) ^ (lane & 7)) << 4)) =
+                  make_uint4(y[0], y[1], y[2], y[3]);
             }
           }
+          __syncwarp();
+          const int piece = lane & 7;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            const uint64_t row_dst = __shfl_sync(~0u, dst, r);
+            if (((owned >> r) & 1) && c0 + piece * 8 < p.head_dim)
+              *reinterpret_cast<uint4*>(row_dst + (c0 + piece * 8) * sizeof(T)) =
+                  *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+          }
+          __syncwarp();
         }
         if (mine && p.lse) p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, scale, logf(l));
         tc_fence_before();  // these reads of O before the next item's first product into it
