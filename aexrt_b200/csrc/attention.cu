@@ -11,6 +11,7 @@
 
 #include "../../include/aexrt_b200.h"
 #include "attention_rows.cuh"
+#include "attention_tc.cuh"
 #include "kernels_attention.cuh"
 #include "kv_cache.cuh"
 #include "launch.cuh"
@@ -211,7 +212,22 @@ uint32_t rows_grid(const AexrtB200AttentionDesc* d) {
 }
 
 uint64_t rows_workspace(uint64_t grid, uint64_t rows, uint64_t head_dim) {
-  return grid * (sizeof(RowsRun) + 2 * rows * (head_dim + 2) * sizeof(float)) + 16;
+  return grid * (sizeof(JoinHead) + 2 * rows * (head_dim + 2) * sizeof(float)) + 16;
+}
+
+// The joining launch may start while the launch before it ends; it waits for that before it reads anything.
+template <typename... KArgs>
+int launch_join(void (*fn)(KArgs...), dim3 grid, int threads, cudaStream_t st, const std::decay_t<KArgs>&... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, fn, args...), "attention join launch") ? 1 : 0;
 }
 
 int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* workspace, cudaStream_t st) {
@@ -219,7 +235,7 @@ int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* work
   rp.a = p;
   rp.rows = static_cast<int>(few_rows(d));
   const uint32_t grid = rows_grid(d);
-  rp.runs = static_cast<RowsRun*>(workspace);
+  rp.runs = static_cast<JoinHead*>(workspace);
   rp.parts = reinterpret_cast<float*>(rp.runs + grid);
   rp.stats = rp.parts + 2ull * grid * rp.rows * p.head_dim;
   const RowsKernel k = attention_rows_for(d->dtype == AEXRT_B200_DTYPE_BF16, p.head_dim, rp.rows);
@@ -229,23 +245,36 @@ int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* work
   if (!cuda_ok(launch_kernel(k.fn, dim3(grid), dim3(kRowsThreads), k.smem, st, maps[0], maps[1], rp), "attention launch"))
     return 0;
   if (grid == 1) return 1;
-  // the joining launch may start while the runs end; it waits for them before it reads anything
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid - 1);
-  cfg.blockDim = dim3(kRowsCompute);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cuda_ok(cudaLaunchKernelEx(&cfg, k.join, rp), "attention join launch") ? 1 : 0;
+  return launch_join(k.join, dim3(grid - 1), kRowsCompute, st, rp);
 }
 
-int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, cudaStream_t st) {
+// Items of a tensor-core call at most (every sequence ends in at most one partial pair of tiles), and into how many
+// parts each is split: as many as fill the SMs, when the items do not fill half of them and a table row holds
+// enough key tiles.
+uint64_t tc_items(const AexrtB200AttentionDesc* d) {
+  const uint64_t tokens = kTcRows / (d->q_heads / d->kv_heads);
+  uint64_t each = d->num_seqs, rows = d->q_tokens;
+  if (d->max_q) each = std::min<uint64_t>(each + rows / (2 * tokens), each * ((d->max_q + 2 * tokens - 1) / (2 * tokens)));
+  else each += rows / (2 * tokens);
+  return each * d->kv_heads;
+}
+
+uint32_t tc_parts(const AexrtB200AttentionDesc* d) {
+  const uint64_t tiles = (static_cast<uint64_t>(d->table_columns) * d->page_size + kTcKeys - 1) / kTcKeys;
+  const uint64_t parts = std::min<uint64_t>(sm_count() / std::max<uint64_t>(1, tc_items(d)), 32);
+  // without the table's columns (the workspace's size is asked for before there is a table) as for a long one
+  return static_cast<uint32_t>(std::max<uint64_t>(1, d->table_columns ? std::min(parts, tiles / kTcMinTiles) : parts));
+}
+
+uint64_t tc_workspace(const AexrtB200AttentionDesc* d) {
+  const uint64_t parts = tc_parts(d), items = tc_items(d);
+  return parts == 1 ? 0 : items * (sizeof(JoinHead) + parts * 256 * (d->head_dim + 2) * sizeof(float));
+}
+
+int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, void* workspace, cudaStream_t st) {
   const CUtensorMapDataType dt =
       d->dtype == AEXRT_B200_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const uint32_t tokens = kTcTileRows / p.group;
+  const uint32_t tokens = kTcRows / p.group;
   CUtensorMap maps[3];
   {
     const uint64_t dims[4] = {d->head_dim, static_cast<uint64_t>(p.group), d->kv_heads, d->q_tokens};
@@ -253,17 +282,23 @@ int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, 
     const uint32_t box[4] = {64, static_cast<uint32_t>(p.group), 1, tokens};
     if (!encode_tensor_map(&maps[0], dt, 4, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return 0;
   }
-  if (!kv_maps(d, p, paged, kTcTileKeys, maps + 1)) return 0;
-  const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, p.head_dim);
+  if (!kv_maps(d, p, paged, kTcKeys, maps + 1)) return 0;
+  // one block per SM, fewer when there cannot be an item for each
+  const uint64_t items = tc_items(d);
+  TcSplit split = {};
+  split.parts = paged ? static_cast<int>(tc_parts(d)) : 1;
+  if (split.parts > 1) {
+    split.heads = static_cast<JoinHead*>(workspace);
+    split.sums = reinterpret_cast<float*>(split.heads + items);
+    split.stats = split.sums + items * split.parts * 256 * d->head_dim;
+  }
+  const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, split.parts > 1, p.head_dim);
   if (!raise_smem(reinterpret_cast<const void*>(k.fn), k.smem)) return 0;
-  // one block per SM, fewer when there cannot be an item for each: every sequence ends in at most one partial pair of tiles
-  const uint64_t items = (static_cast<uint64_t>(d->q_tokens) / (2 * tokens) + d->num_seqs) * d->kv_heads;
-  const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(items, sm_count()));
-  return cuda_ok(launch_kernel(k.fn, dim3(blocks), dim3(kTcBlock), k.smem, st, maps[0], maps[1],
-                               maps[2], p),
-                 "attention launch")
-             ? 1
-             : 0;
+  const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(items * split.parts, sm_count()));
+  if (!cuda_ok(launch_kernel(k.fn, dim3(blocks), dim3(kTcThreads), k.smem, st, maps[0], maps[1], maps[2], p, split),
+               "attention launch"))
+    return 0;
+  return split.parts == 1 ? 1 : launch_join(k.join, dim3(static_cast<unsigned>(items), 256 / kTcJoinRows), kTcJoinThreads, st, p, split);
 }
 
 }  // namespace
@@ -280,14 +315,14 @@ int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, 
   p.status = status_word();
   if (!p.status) return 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return launch_tc(d, p, false, st);
+  return launch_tc(d, p, false, nullptr, st);
 }
 
 uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* d) {
   if (!desc_ok(d, true)) return ~0ull;
   if (d->q_tokens == 0 || d->num_seqs == 0 || d->max_q == 0) return 0;
   const uint32_t rows = few_rows(d);
-  return rows ? rows_workspace(2ull * sm_count(), rows, d->head_dim) : 0;
+  return rows ? rows_workspace(2ull * sm_count(), rows, d->head_dim) : tc_workspace(d);
 }
 
 int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, const void* k_cache, const void* v_cache,
@@ -311,7 +346,7 @@ int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, c
   p.status = status_word();
   if (!p.status) return 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return few_rows(d) ? launch_rows(d, p, workspace, st) : launch_tc(d, p, true, st);
+  return few_rows(d) ? launch_rows(d, p, workspace, st) : launch_tc(d, p, true, workspace, st);
 }
 
 int aexrt_b200_attention_status(uint32_t* status) {

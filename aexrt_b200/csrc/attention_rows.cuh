@@ -16,7 +16,7 @@
 #pragma once
 #include <climits>
 
-#include "attention_math.cuh"
+#include "attention_join.cuh"
 
 namespace aexrt {
 
@@ -37,16 +37,9 @@ struct RowsSmem {
   static constexpr int kBytes = kBars + 2 * rows_stages<DP>() * 8;
 };
 
-// What a run leaves for the joining when it is the first to go on with a (sequence, head) that the run
-// before it began: the parts it is in (this run's predecessor's, its own and its successors'; 0:
-// nothing to join), its query rows and where they lie.
-struct RowsRun {
-  int parts, rows, q0, head;
-};
-
 struct RowsParams {
   AttnParams a;
-  RowsRun* runs;    // [grid]
+  JoinHead* runs;   // [grid]: of the (sequence, head) that run c goes on with, when it is the first to do so
   float* parts;     // [grid][2][rows][head_dim]: first a run's part of a (sequence, head) begun before it, then of one that goes on behind it
   float* stats;     // [grid][2][rows][2]: maximum (raw score units), normaliser
   int rows;         // max_q * group
@@ -227,7 +220,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       // is this run the first that goes on with its first (sequence, head)?  Then it heads the joining.
       const int c = blockIdx.x;
       const int64_t first = start - begin.tile, end = first + begin.tiles;
-      RowsRun r = {};
+      JoinHead r = {};
       if (begin.tile > 0 && cut.start(c - 1) <= first) {
         r.parts = 1;
         while (c + r.parts - 1 < cut.runs && cut.start(c + r.parts - 1) < end) ++r.parts;
@@ -489,58 +482,21 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 }
 
 // Joins the parts of every (sequence, head) that was cut: block c - 1 takes the one that run c heads.
-// A thread has 8 columns of a row; parts are summed in the order of the keys.
+// A thread has 8 columns of a row.
 template <typename T>
 __global__ void __launch_bounds__(kRowsCompute) attention_rows_join_kernel(const RowsParams rp) {
   grid_dep_launch();
   grid_dep_wait();
   const AttnParams& p = rp.a;
   const int c = blockIdx.x + 1;
-  const RowsRun run = rp.runs[c];
+  const JoinHead run = rp.runs[c];
   if (run.parts == 0) return;
-  const float scale = fmaxf(p.scale, 1e-30f), sl2 = scale * 1.4426950408889634f;
   const int vecs = p.head_dim / 8;
   for (int i = threadIdx.x; i < run.rows * vecs; i += kRowsCompute) {
-    const int r = i / vecs, d = i % vecs * 8;
+    const int r = i / vecs;
     // part k is run c - 1 + k's: the second slot of the first run, the first slot of the others
     auto row_of = [&](int k) { return (static_cast<int64_t>(2 * (c - 1 + k) + (k == 0 ? 1 : 0))) * rp.rows + r; };
-    float y[8] = {}, all = -INFINITY, norm = 0.f;
-    for (int k0 = 0; k0 < run.parts; k0 += 4) {  // four parts' loads at a time
-      float2 st[4];
-      float4 a[4], b[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t row = row_of(min(k0 + k, run.parts - 1));
-        st[k] = *reinterpret_cast<const float2*>(rp.stats + row * 2);
-        const float4* src = reinterpret_cast<const float4*>(rp.parts + row * p.head_dim + d);
-        a[k] = src[0];
-        b[k] = src[1];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (k0 + k >= run.parts) break;
-        if (st[k].x > all) {  // a new maximum: what is summed so far shrinks
-          const float f = all == -INFINITY ? 0.f : exp2_sfu((all - st[k].x) * sl2);
-          norm *= f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = f == 0.f && !isfinite(y[e]) ? y[e] : y[e] * f;
-          all = st[k].x;
-        }
-        const float f = st[k].x == all ? 1.f : (st[k].x == -INFINITY ? 0.f : exp2_sfu((st[k].x - all) * sl2));
-        norm = fmaf(st[k].y, f, norm);
-        const float x[8] = {a[k].x, a[k].y, a[k].z, a[k].w, b[k].x, b[k].y, b[k].z, b[k].w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = f == 0.f && !isfinite(x[e]) ? y[e] + x[e] : fmaf(x[e], f, y[e]);
-      }
-    }
-    const float inv = norm == 0.f ? 0.f : 1.f / norm;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] *= inv;
-    const int token = run.q0 + r / p.group, qh = run.head * p.group + r % p.group;
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + token * p.o_ts + qh * p.o_hs + d) =
-        make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
-    if (d == 0 && p.lse)
-      p.lse[static_cast<int64_t>(token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
+    join_row<T>(p, rp.parts, rp.stats, run.parts, row_of, i % vecs * 8, run.q0 + r / p.group, run.head * p.group + r % p.group);
   }
 }
 

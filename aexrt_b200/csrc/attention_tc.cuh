@@ -18,6 +18,9 @@
 // two products at head size 128.  Taking a part of the powers by a polynomial on the multiply-add
 // pipes instead made every size slower (8 of 32: 3 %, 16 of 32: 8 %): the softmax warps are not what the products wait for.
 //
+// When there are too few items for the SMs, and a workspace (the paged cache), an item's key tiles are split
+// over several CTAs; each leaves its rows' unnormalised sums, and a second launch joins them.
+//
 // One CTA per SM stays for all its items: the loads, the score products and the search of the next
 // item go on while the softmax warps write the last one's output.  Items go out in the order of their key tiles,
 // the longest first, one to each CTA in turn and every other turn backwards, so that ragged batches
@@ -32,13 +35,15 @@
 #pragma once
 #include <climits>
 
-#include "attention_math.cuh"
+#include "attention_join.cuh"
 
 namespace aexrt {
 
 constexpr int kTcRows = 128;   // query rows of a tile
 constexpr int kTcKeys = 128;   // keys of a tile
 constexpr int kTcThreads = 384;
+// Key tiles of a part at least: with 2 the joining costs 300 cached keys 22 instead of 19 us, with 8 2000 keys take 33 instead of 28.
+constexpr int kTcMinTiles = 4;
 
 // Slots of the K / V ring: what 227 KB hold beside the two Q tiles and the output staging.
 template <int DP>
@@ -50,7 +55,7 @@ struct TcSmem {
   static constexpr int kQ = 0, kRing = 2 * kTile, kStage = kRing + tc_slots<DP>() * kTile;
   static constexpr int kBars = kStage + 8 * 4096;  // per softmax warp: 32 rows of 64 output columns
   // barriers, TMEM base, items; then, per item of two, the first keys with non-finite values of a column
-  static constexpr int kFix = kBars + 512, kBytes = kFix + 2 * kFixInts * 4;
+  static constexpr int kFix = kBars + 640, kBytes = kFix + 2 * kFixInts * 4;
 };
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
@@ -104,6 +109,16 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 struct TcWork {
   int head, seq, tile, len_q, rows_q, len_k, q0, k0;  // rows_q: query tokens taken (len_q, at most max_q); head -1: no more
+  int begin, end;  // key tiles
+  int part;        // part of the workspace that the rows go to, -1: the item is whole
+};
+
+// Splitting: the most parts of an item, and where they go.
+struct TcSplit {
+  int parts;       // 1: none
+  JoinHead* heads; // [items]
+  float* sums;     // [items][parts][256][head_dim]
+  float* stats;    // [items][parts][256][2]
 };
 
 // Numbers the items of a call: descending in key tiles while a warp can hold every sequence's lengths
@@ -232,18 +247,19 @@ struct TcFinder {
   }
 };
 
-// An item's two row tiles: first token, tokens, keys that the last one sees, key tiles.
+// An item's two row tiles: first token, tokens, keys that the last one sees, key tiles from `begin` on.
+template <bool kSplit>
 struct TcTiles {
-  int first[2], valid[2], n[2];
+  int first[2], valid[2], keys[2], n[2];
   int key_end, nmax, common;  // keys at and above `common` are seen by some rows and not by others
   __device__ __forceinline__ TcTiles(const AttnParams& p, const TcWork& w, int tokens) {
-    int keys[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       first[s] = (w.tile * 2 + s) * tokens;
       valid[s] = clampi(w.rows_q - first[s], 0, tokens);
       keys[s] = valid[s] ? keys_seen(first[s] + valid[s] - 1, w.len_q, w.len_k, p.causal) : 0;
       n[s] = (keys[s] + kTcKeys - 1) / kTcKeys;
+      if (kSplit) n[s] = max(0, min(n[s], w.end) - w.begin);
     }
     key_end = max(keys[0], keys[1]);
     nmax = max(n[0], n[1]);
@@ -256,27 +272,32 @@ __device__ __forceinline__ void mbar_arrive_count(uint64_t* bar, uint32_t count)
                : "memory");
 }
 
+// Quarters of 32 keys that a row tile needs of key tile j when its last row sees `keys` keys: products and
+// softmax of the last tile stop there.
+__device__ __forceinline__ int tc_quarters(int keys, int j) { return min(4, (keys - j * kTcKeys + 31) >> 5); }
+
 template <int kRegs>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
-template <typename T, bool kPaged, int DP>
+template <typename T, bool kPaged, int DP, bool kSplit>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attention_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                        const __grid_constant__ CUtensorMap v_map, const AttnParams p) {
+                        const __grid_constant__ CUtensorMap v_map, const AttnParams p, const TcSplit split) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using L = TcSmem<DP>;
   constexpr int NS = tc_slots<DP>(), kHalves = DP / 64;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t *q_empty = q_full + 2, *s_full = q_empty + 2, *p_full = s_full + 2, *o_done = p_full + 2, *w_full = o_done + 2,
-           *w_empty = w_full + 2, *kv_full = w_empty + 2, *kv_empty = kv_full + NS, *raw = kv_empty + NS, *s_free = raw + 1,
+           *w_empty = w_full + 2, *kv_full = w_empty + 2, *kv_empty = kv_full + NS, *raw = kv_empty + NS, *s_free = raw + NS,
            *drain = s_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* fixed = reinterpret_cast<int*>(tmem_slot + 1);  // [2]
   TcWork* work = reinterpret_cast<TcWork*>(fixed + 3);  // [2]
+  int4* unclean = reinterpret_cast<int4*>((reinterpret_cast<uintptr_t>(work + 2) + 15) & ~uintptr_t{15});  // [NS], see the loads
   int* fix = reinterpret_cast<int*>(smem + L::kFix);    // [2][kFixInts]
-  static_assert((14 + 2 * tc_slots<DP>() + 5) * 8 + 16 + 2 * sizeof(TcWork) <= 512, "barriers and items fit");
+  static_assert((14 + 3 * tc_slots<DP>() + 4) * 8 + 16 + 2 * sizeof(TcWork) + 16 * tc_slots<DP>() <= 640, "barriers and items fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dep_launch();
@@ -296,8 +317,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int i = 0; i < NS; ++i) {
       mbar_init(kv_full + i, 1);
       mbar_init(kv_empty + i, 2);
+      mbar_init(raw + i, 1);
     }
-    mbar_init(raw, 1);
     fence_mbar_init();
   }
   for (int i = threadIdx.x; i < 2 * kFixInts; i += kTcThreads) fix[i] = INT_MAX;
@@ -326,9 +347,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       TcFinder<kPaged> finder(p, 2 * tokens);
       for (int k = 0;; ++k) {
         const int64_t number = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const int64_t rest = number / p.kv_heads, number_of = kSplit ? rest / split.parts : rest;
         TcWork w = {};
-        const bool found = finder.find(number / p.kv_heads, w);
-        w.head = found ? static_cast<int>(number % p.kv_heads) : -1;
+        w.end = INT_MAX;
+        w.part = -1;
+        bool found = finder.find(number_of, w);
+        w.head = static_cast<int>(number % p.kv_heads);
+        if constexpr (kSplit) {  // one number per CTA
+          const int part = static_cast<int>(rest % split.parts);
+          const int64_t slot = number_of * p.kv_heads + w.head;
+          JoinHead head = {};
+          if (found) {
+            const TcTiles<kSplit> t(p, w, tokens);
+            const int parts = clampi(t.nmax / kTcMinTiles, 1, split.parts);
+            if (parts > 1) {
+              head = JoinHead{parts, t.valid[0] + t.valid[1], w.q0 + t.first[0], w.head};
+              w.begin = static_cast<int>(static_cast<int64_t>(t.nmax) * part / parts);
+              w.end = static_cast<int>(static_cast<int64_t>(t.nmax) * (part + 1) / parts);
+              w.part = static_cast<int>(slot * split.parts + part);
+            }
+            found = part < parts;
+          }
+          if (part == 0 && lane == 0 && slot * split.parts < gridDim.x) split.heads[slot] = head;
+        }
+        if (!found) w.head = -1;
         if (!__all_sync(~0u, wait(w_empty + (k & 1), (k >> 1) + 1))) break;
         if (lane == 0) {
           work[k & 1] = w;
@@ -340,60 +382,60 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // ---------------------------------------------------------------- loads
       const uint32_t q_bytes = static_cast<uint32_t>(tokens * p.group * 128 * kHalves);
       bool ok = true;
-      int raws = 0, it = 0, qs[2] = {0, 0};
-      // A V tile that has to be cleaned before its product.  P is 0 where a row does not see a key, but
-      // 0 * inf and 0 * NaN are not: rows behind the last key become zeros, and non-finite values of
-      // keys that only some rows see are taken out and put back into the outputs of the rows that do.
-      // The tile lands on a barrier of its own and is cleaned while later loads are already on their way.
-      bool dirty = false;
-      int d_slot = 0, d_item = 0, d_from = 0, d_last = 0, d_key = 0;  // rows from .. last are looked at
-      bool d_release = false;  // the item has no other loads left
+      int it = 0, qs[2] = {0, 0};
+      // V tiles that have to be cleaned before their product.  P is 0 where a row does not see a key, but
+      // 0 * inf and 0 * NaN are not: rows behind the last key become zeros (as far as the product goes, a
+      // quarter of the tile), and non-finite values of keys that only some rows see are taken out and put
+      // back into the outputs of the rows that do.  Such a tile lands on a barrier of its own and is cleaned
+      // while later loads are already on their way.
+      // Of a slot's tile: x, y the rows that are looked at (from, last), z its first key, w its item, and
+      // whether that has no loads after it (bit 31).  `queue`: slots in order, 4 bits each.
+      uint32_t queue = 0, waiting = 0, raws = 0;  // raws: per slot, the phase of its barrier
       auto clean = [&]() {
-        uint8_t* dst = smem + L::kRing + d_slot * L::kTile;
-        int* fx = fix + (d_item & 1) * kFixInts;
+        const int slot = queue & 15;
+        __syncwarp();
+        const int4 u = unclean[slot];
+        const int from = u.x, last = u.y, of = u.w & 1;
+        uint8_t* dst = smem + L::kRing + slot * L::kTile;
+        int* fx = fix + of * kFixInts;
         const int sub = lane >> 3, piece = lane & 7;  // 16-byte piece c of row r lies at piece c ^ (r % 8): the 128-byte swizzle
         for (int h = 0; h < kHalves; ++h) {
           uint4* tile = reinterpret_cast<uint4*>(dst + h * 16384) + piece;
 #pragma unroll 4
-          for (int r = d_last + sub; r < kTcKeys; r += 4) tile[r * 8] = make_uint4(0, 0, 0, 0);
-          for (int r = d_from + sub; r < d_last; r += 32) {
+          for (int r = last + sub; r < min(kTcKeys, (last + 31) & ~31); r += 4) tile[r * 8] = make_uint4(0, 0, 0, 0);
+          for (int r = from + sub; r < last; r += 32) {
             uint32_t bits = 0;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {  // rows past the end look at this lane's first row again
-              const uint4 x = tile[(r + 4 * u < d_last ? r + 4 * u : r) * 8];
+            for (int i = 0; i < 8; ++i) {  // rows past the end look at this lane's first row again
+              const uint4 x = tile[(r + 4 * i < last ? r + 4 * i : r) * 8];
               bits |= non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w);
             }
             if (bits) {
-              for (int row = r; row < min(r + 32, d_last); row += 4)
-                tile[row * 8] = take_non_finite<T>(tile[row * 8], d_key + row, h * 64 + (piece ^ (row & 7)) * 8, fx);
-              fixed[d_item & 1] = 1;
+              for (int row = r; row < min(r + 32, last); row += 4)
+                tile[row * 8] = take_non_finite<T>(tile[row * 8], u.z + row, h * 64 + (piece ^ (row & 7)) * 8, fx);
+              fixed[of] = 1;
             }
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(kv_full + d_slot);
-          if (d_release) mbar_arrive(w_empty + (d_item & 1));
+          mbar_arrive(kv_full + slot);
+          if (u.w < 0) mbar_arrive(w_empty + of);
         }
-        dirty = d_release = false;
+        raws ^= 1u << slot;
+        queue >>= 4;
+        --waiting;
       };
-      auto flush = [&]() {  // the tile to be cleaned, now
-        if (dirty && ok) {
-          ok = __all_sync(~0u, wait(raw, raws++));
-          if (ok) clean();
-        }
-      };
-      auto wait_serving = [&](uint64_t* bar, int phase) {  // a wait that cleans the tile when that lands first
+      auto wait_serving = [&](uint64_t* bar, int phase) {  // a wait that cleans what lands first
         const long long t0 = clock64();
-        while (dirty) {
+        while (waiting) {
           if (__any_sync(~0u, mbar_test_wait(bar, phase & 1))) return true;
-          if (__any_sync(~0u, mbar_test_wait(raw, raws & 1))) {
-            ++raws;
+          const int slot = queue & 15;
+          if (__any_sync(~0u, mbar_test_wait(raw + slot, (raws >> slot) & 1)))
             clean();
-          } else if (__any_sync(~0u, clock64() - t0 > kWaitLimitCycles)) {
+          else if (__any_sync(~0u, clock64() - t0 > kWaitLimitCycles))
             break;
-          }
         }
         return __all_sync(~0u, wait(bar, phase)) != 0;
       };
@@ -402,7 +444,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ok = wait_serving(w_full + (k & 1), k >> 1);
         w = work[k & 1];
         if (!ok || w.head < 0) break;
-        const TcTiles t(p, w, tokens);
+        const TcTiles<kSplit> t(p, w, tokens);
         if (fixed[k & 1]) {  // the roles have left the item that used it last
           __syncwarp();
           for (int i = lane; i < kFixInts; i += 32) fix[(k & 1) * kFixInts + i] = INT_MAX;
@@ -439,42 +481,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           __syncwarp();
         };
+        bool released = false;
         load_q(0);
         for (int i = 0; i < 2 * t.nmax && ok; ++i, ++it) {  // K0 K1 V0 K2 V1 ... as the products take them
           const bool is_v = i + 1 == 2 * t.nmax || (i > 0 && !(i & 1));
-          const int slot = it % NS, j = is_v ? (i + 1 == 2 * t.nmax ? t.nmax : i >> 1) - 1 : (i + 1) >> 1;
+          const int slot = it % NS, j = (kSplit ? w.begin : 0) + (is_v ? (i + 1 == 2 * t.nmax ? t.nmax : i >> 1) - 1 : (i + 1) >> 1);
           const int last = t.key_end - j * kTcKeys, seen = t.common - j * kTcKeys;  // rows of this tile below them
-          const bool unclean = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
-          if (unclean) flush();
-          ok = ok && wait_serving(kv_empty + slot, it / NS + 1);
+          const bool dirty = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
+          ok = wait_serving(kv_empty + slot, it / NS + 1);
           if (!ok) break;
-          load_kv(is_v ? &v_map : &k_map, smem + L::kRing + slot * L::kTile, unclean ? raw : kv_full + slot, j);
+          load_kv(is_v ? &v_map : &k_map, smem + L::kRing + slot * L::kTile, dirty ? raw + slot : kv_full + slot, j);
           if (i == 0) load_q(1);
-          if (unclean) {
-            dirty = true;
-            d_slot = slot;
-            d_item = k;
-            d_last = min(last, kTcKeys);
-            d_from = max(0, min(seen, d_last));
-            d_key = j * kTcKeys;
+          if (dirty) {
+            const int to = min(last, kTcKeys);
+            const bool ends = i + 1 == 2 * t.nmax;
+            if (lane == 0) unclean[slot] = make_int4(max(0, min(seen, to)), to, j * kTcKeys, (k & 1) | (ends ? INT_MIN : 0));
+            queue |= static_cast<uint32_t>(slot) << (4 * waiting++);
+            released = ends;
           }
         }
         __syncwarp();
-        if (dirty && d_item == k) d_release = true;
-        else if (lane == 0) mbar_arrive(w_empty + (k & 1));
+        if (!released && lane == 0) mbar_arrive(w_empty + (k & 1));  // else when its last tile has been cleaned
       }
-      flush();
+      while (waiting && ok) {
+        const int slot = queue & 15;
+        ok = __all_sync(~0u, wait(raw + slot, (raws >> slot) & 1));
+        if (ok) clean();
+      }
       if (!ok) {
         // a wait gave up: the loads in flight still have to land before the CTA may leave
-        for (int i = 0; i < 2 * (NS + 3); ++i) {
-          uint64_t* bar = i < 2 * NS ? kv_full + (i >> 1) : (i < 2 * NS + 4 ? q_full + ((i - 2 * NS) >> 1) : raw);
-          mbar_wait_bounded(bar, i & 1, p.status, kAttnTimeout);
-        }
+        for (uint64_t* bar : {kv_full, raw, q_full})
+          for (int i = 0; i < (bar == q_full ? 2 : NS); ++i) {
+            mbar_wait_bounded(bar + i, 0, p.status, kAttnTimeout);
+            mbar_wait_bounded(bar + i, 1, p.status, kAttnTimeout);
+          }
       }
     } else if (lane == 0) {
       // ---------------------------------------------------------------- MMA issue, one thread per row tile
       const int s = warp == 8 ? 0 : 1;
-      const uint32_t id_s = tc_idesc<T>(kTcKeys, false), id_o = tc_idesc<T>((p.head_dim + 15) / 16 * 16, true);
+      const uint32_t id_s = tc_idesc<T>(kTcKeys, false), id_n = tc_idesc<T>(32, false) - tc_idesc<T>(0, false), id_o = tc_idesc<T>((p.head_dim + 15) / 16 * 16, true);
       const int steps = (p.head_dim + 15) / 16;
       // descriptors of the first K step; later steps and slots add to the address field
       const uint64_t q_desc = desc_sw128(smem_u32(smem + L::kQ + s * L::kTile), 16, 1024);
@@ -486,8 +531,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       auto full = [&](int i) { return wait(kv_full + i % NS, i / NS); };
       TcWork w;
       for (int k = 0; ok && item(k, w); ++k) {
-        const TcTiles t(p, w, tokens);
-        const int n = s ? t.n[1] : t.n[0];
+        const TcTiles<kSplit> t(p, w, tokens);
+        const int n = s ? t.n[1] : t.n[0], keys = s ? t.keys[1] : t.keys[0], begin = kSplit ? w.begin : 0;
         // every ring item in order, K0 K1 V0 K2 V1 ..., also those that only the other tile uses
         for (int j = -1; j < t.nmax && ok; ++j) {
           if (j + 1 < t.nmax) {  // S = Q K^T for key tile j + 1
@@ -502,10 +547,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (j + 1 < n) {
               tc_fence_after();
               const uint64_t b = k_desc + (i % NS) * (L::kTile >> 4);
+              const uint32_t id = id_s - (4 - tc_quarters(keys, begin + j + 1)) * id_n;
 #pragma unroll
               for (int c = 0; c < DP / 16; ++c) {
                 const int off = ((c >> 2) * 16384 + (c & 3) * 32) >> 4;
-                if (c < steps) tc_mma<true>(tmem, q_desc + off, b + off, id_s, c != 0);
+                if (c < steps) tc_mma<true>(tmem, q_desc + off, b + off, id, c != 0);
               }
               tc_commit(s_full + s);
               tc_commit(kv_empty + i % NS);
@@ -523,9 +569,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (!ok) break;
               tc_fence_after();
               const uint64_t b = v_desc + (i % NS) * (L::kTile >> 4);
+              const int quarters = tc_quarters(keys, begin + j);
 #pragma unroll
               for (int c = 0; c < kTcKeys / 16; ++c)
-                tc_mma_ts(o_at, p_at + c * 8, b + c * (2048 >> 4), id_o, (j | c) != 0);
+                if (c < quarters * 2) tc_mma_ts(o_at, p_at + c * 8, b + c * (2048 >> 4), id_o, (j | c) != 0);
               tc_commit(o_done + s);
               tc_commit(kv_empty + i % NS);
             } else if (ok) {
@@ -556,9 +603,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int done = 0;  // key tiles of this row tile so far, over all items
     TcWork w;
     for (int k = 0; ok && __all_sync(~0u, item(k, w)); ++k) {
-      const TcTiles t(p, w, tokens);
+      const TcTiles<kSplit> t(p, w, tokens);
       const int first = s ? t.first[1] : t.first[0], valid = s ? t.valid[1] : t.valid[0], n = s ? t.n[1] : t.n[0];
-      const int token = first + row_token;
+      const int token = first + row_token, begin = kSplit ? w.begin : 0;
       const bool mine = row_token < valid;  // rows behind the last whole token have row_token >= tokens
       const int seen = mine ? keys_seen(token, w.len_q, w.len_k, p.causal) : 0;
       const int all_see = valid ? keys_seen(first, w.len_q, w.len_k, p.causal) : 0;
@@ -573,11 +620,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive(s_free + s);
-        if ((j + 1) * kTcKeys > all_see) {
-          const int lim = seen - j * kTcKeys;
+        if ((begin + j + 1) * kTcKeys > all_see) {
+          const int lim = seen - (begin + j) * kTcKeys;
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= lim) x[c] = 0xff800000u;
+          for (int c = 0; c < 4; ++c) {
+            // bit i: the row sees column 32 c + i (columns that the product left out are never seen)
+            const uint32_t sees = lim >= 32 * c + 32 ? ~0u : (lim <= 32 * c ? 0u : (1u << (lim - 32 * c)) - 1u);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(sees & (1u << e))) x[32 * c + e] = 0xff800000u;
+          }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -636,7 +688,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (ok && n) ok = __all_sync(~0u, wait(o_done + s, done - 1));
       if (ok && valid) {
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const bool part = kSplit && w.part >= 0;
+        const float inv = part ? 1.f : (l == 0.f ? 0.f : 1.f / l);
         const int64_t tok = w.q0 + token;
         const int qh = w.head * p.group + row_head;
         const uint64_t dst = reinterpret_cast<uint64_t>(static_cast<T*>(p.out) + tok * p.o_ts + qh * p.o_hs);
@@ -646,7 +699,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // 64 columns at a time through shared memory (16-byte piece c of row r at c ^ (r % 8)): a store
         // instruction then writes whole 128-byte lines of four rows instead of 16 bytes of 32
         uint8_t* stage = smem + L::kStage + warp * 4096;
-        for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
+        for (int c0 = 0; c0 < p.head_dim && !part; c0 += 64) {
           for (int c = c0; c < min(c0 + 64, p.head_dim); c += 32) {
             uint32_t o[32];
             if (n) {
@@ -683,17 +736,59 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           __syncwarp();
           const int piece = lane & 7;
+          uint4 y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            y[i] = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = 4 * i + (lane >> 3);
             const uint64_t row_dst = __shfl_sync(~0u, dst, r);
             if (((owned >> r) & 1) && c0 + piece * 8 < p.head_dim)
-              *reinterpret_cast<uint4*>(row_dst + (c0 + piece * 8) * sizeof(T)) =
-                  *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+              *reinterpret_cast<uint4*>(row_dst + (c0 + piece * 8) * sizeof(T)) = y[i];
           }
           __syncwarp();
         }
-        if (mine && p.lse) p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, scale, logf(l));
+        if (kSplit && part) {  // fp32 sums, 32 columns at a time through the same staging
+          float* sums = split.sums + (static_cast<int64_t>(w.part) * 256 + s * 128 + (warp & 3) * 32) * p.head_dim;
+          for (int c = 0; c < p.head_dim; c += 32) {
+            uint32_t o[32];
+            if (n) {
+              tmem_ld_32x32(o_at + c, o);
+              tmem_ld_wait();
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = n && seen ? o[e] : 0u;
+            if (patch) {
+#pragma unroll 1
+              for (int e = 0; e < 32; ++e) {
+                const float y = put_back(__uint_as_float(o[0]), fx, c + e, seen);
+#pragma unroll
+                for (int i = 0; i < 31; ++i) o[i] = o[i + 1];
+                o[31] = __float_as_uint(y);
+              }
+            }
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((v ^ (lane & 7)) << 4)) =
+                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            __syncwarp();
+            const int piece = lane & 7;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              if (((owned >> r) & 1) && c + piece * 4 < p.head_dim)
+                *reinterpret_cast<uint4*>(sums + r * p.head_dim + c + piece * 4) =
+                    *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+            }
+            __syncwarp();
+          }
+          if (mine) *reinterpret_cast<float2*>(split.stats + (static_cast<int64_t>(w.part) * 256 + s * 128 + row) * 2) = make_float2(m, l);
+        } else if (mine && p.lse) {
+          p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, scale, logf(l));
+        }
         tc_fence_before();  // these reads of O before the next item's first product into it
       }
       __syncwarp();
@@ -705,6 +800,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the split items: a block takes 16 of an item's 256 rows, a thread 8 columns of a row.
+constexpr int kTcJoinThreads = 256, kTcJoinRows = 16;
+template <typename T>
+__global__ void __launch_bounds__(kTcJoinThreads) attention_tc_join_kernel(const AttnParams p, const TcSplit split) {
+  grid_dep_launch();
+  grid_dep_wait();
+  const JoinHead item = split.heads[blockIdx.x];
+  if (item.parts == 0) return;
+  const int tokens = kTcRows / p.group, vecs = p.head_dim / 8;
+  for (int i = threadIdx.x; i < kTcJoinRows * vecs; i += kTcJoinThreads) {
+    const int r = blockIdx.y * kTcJoinRows + i / vecs, in_tile = r & 127, row_token = in_tile / p.group;
+    const int token = (r >> 7) * tokens + row_token;
+    if (row_token >= tokens || token >= item.rows) continue;
+    auto row_of = [&](int k) { return (static_cast<int64_t>(blockIdx.x) * split.parts + k) * 256 + r; };
+    join_row<T>(p, split.sums, split.stats, item.parts, row_of, i % vecs * 8, item.q0 + token, item.head * p.group + in_tile % p.group);
   }
 }
 
