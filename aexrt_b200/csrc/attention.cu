@@ -248,27 +248,45 @@ int launch_rows(const AexrtB200AttentionDesc* d, const AttnParams& p, void* work
   return launch_join(k.join, dim3(grid - 1), kRowsCompute, st, rp);
 }
 
-// Items of a tensor-core call at most (every sequence ends in at most one partial pair of tiles), and into how many
-// parts each is split: as many as fill the SMs, when the items do not fill half of them and a table row holds
-// enough key tiles.
+// Items of a tensor-core call at most: every sequence ends in at most one partial pair of tiles.
 uint64_t tc_items(const AexrtB200AttentionDesc* d) {
   const uint64_t tokens = kTcRows / (d->q_heads / d->kv_heads);
-  uint64_t each = d->num_seqs, rows = d->q_tokens;
-  if (d->max_q) each = std::min<uint64_t>(each + rows / (2 * tokens), each * ((d->max_q + 2 * tokens - 1) / (2 * tokens)));
-  else each += rows / (2 * tokens);
+  uint64_t each = d->num_seqs + static_cast<uint64_t>(d->q_tokens) / (2 * tokens);
+  if (d->max_q) each = std::min<uint64_t>(each, d->num_seqs * ((d->max_q + 2 * tokens - 1) / (2 * tokens)));
   return each * d->kv_heads;
 }
 
-uint32_t tc_parts(const AexrtB200AttentionDesc* d) {
-  const uint64_t tiles = (static_cast<uint64_t>(d->table_columns) * d->page_size + kTcKeys - 1) / kTcKeys;
-  const uint64_t parts = std::min<uint64_t>(sm_count() / std::max<uint64_t>(1, tc_items(d)), 32);
-  // without the table's columns (the workspace's size is asked for before there is a table) as for a long one
-  return static_cast<uint32_t>(std::max<uint64_t>(1, d->table_columns ? std::min(parts, tiles / kTcMinTiles) : parts));
+// Whether a paged call's items are split over their keys: when there are at most 3 for every 2 SMs (beyond that they even
+// out by themselves; two requests of 1024 tokens, 272 items, gain nothing) and a table row can hold keys for two parts.
+// Without the table's columns (the workspace's size is asked for before there is a table) as for a long row.
+bool tc_splits(const AexrtB200AttentionDesc* d) {
+  const uint64_t keys = static_cast<uint64_t>(d->table_columns) * d->page_size;
+  return 2 * tc_items(d) <= 3 * static_cast<uint64_t>(sm_count()) && (d->table_columns == 0 || keys >= 2ull * kTcMinTiles * kTcKeys);
+}
+
+// Lays a split call's workspace out (from null: its size).
+TcSplit tc_split(void* workspace, uint64_t head_dim, uint64_t* bytes) {
+  const uint64_t grid = sm_count(), parts = 3 * grid;
+  TcSplit split = {};
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  auto take = [&](uint64_t n) {
+    uint8_t* here = at;
+    at += (n + 15) / 16 * 16;
+    return here;
+  };
+  split.split_items = reinterpret_cast<int*>(take(sizeof(int)));
+  split.bases = reinterpret_cast<int*>(take(parts * sizeof(int)));
+  split.heads = reinterpret_cast<JoinHead*>(take(2 * grid * sizeof(JoinHead)));
+  split.sums = reinterpret_cast<float*>(take(parts * 256 * head_dim * sizeof(float)));
+  split.stats = reinterpret_cast<float*>(take(parts * 256 * 2 * sizeof(float)));
+  *bytes = static_cast<uint64_t>(at - static_cast<uint8_t*>(workspace));
+  return split;
 }
 
 uint64_t tc_workspace(const AexrtB200AttentionDesc* d) {
-  const uint64_t parts = tc_parts(d), items = tc_items(d);
-  return parts == 1 ? 0 : items * (sizeof(JoinHead) + parts * 256 * (d->head_dim + 2) * sizeof(float));
+  uint64_t bytes = 0;
+  if (tc_splits(d)) tc_split(nullptr, d->head_dim, &bytes);
+  return bytes;
 }
 
 int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, void* workspace, cudaStream_t st) {
@@ -283,22 +301,18 @@ int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, 
     if (!encode_tensor_map(&maps[0], dt, 4, p.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return 0;
   }
   if (!kv_maps(d, p, paged, kTcKeys, maps + 1)) return 0;
-  // one block per SM, fewer when there cannot be an item for each
-  const uint64_t items = tc_items(d);
-  TcSplit split = {};
-  split.parts = paged ? static_cast<int>(tc_parts(d)) : 1;
-  if (split.parts > 1) {
-    split.heads = static_cast<JoinHead*>(workspace);
-    split.sums = reinterpret_cast<float*>(split.heads + items);
-    split.stats = split.sums + items * split.parts * 256 * d->head_dim;
-  }
-  const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, split.parts > 1, p.head_dim);
+  const bool splits = paged && tc_splits(d);
+  uint64_t bytes = 0;
+  const TcSplit split = splits ? tc_split(workspace, d->head_dim, &bytes) : TcSplit{};
+  const TcKernel k = attention_tc_for(d->dtype == AEXRT_B200_DTYPE_BF16, paged, splits, p.head_dim);
   if (!raise_smem(reinterpret_cast<const void*>(k.fn), k.smem)) return 0;
-  const unsigned blocks = static_cast<unsigned>(std::min<uint64_t>(items * split.parts, sm_count()));
+  // one block per SM, fewer when there cannot be an item for each
+  const unsigned sms = static_cast<unsigned>(sm_count());
+  const unsigned blocks = splits ? sms : static_cast<unsigned>(std::min<uint64_t>(tc_items(d), sms));
   if (!cuda_ok(launch_kernel(k.fn, dim3(blocks), dim3(kTcThreads), k.smem, st, maps[0], maps[1], maps[2], p, split),
                "attention launch"))
     return 0;
-  return split.parts == 1 ? 1 : launch_join(k.join, dim3(static_cast<unsigned>(items), 256 / kTcJoinRows), kTcJoinThreads, st, p, split);
+  return splits ? launch_join(k.join, dim3((sms + 1) / 2, 256 / kTcJoinRows), kTcJoinThreads, st, p, split) : 1;
 }
 
 }  // namespace

@@ -18,8 +18,9 @@
 // two products at head size 128.  Taking a part of the powers by a polynomial on the multiply-add
 // pipes instead made every size slower (8 of 32: 3 %, 16 of 32: 8 %): the softmax warps are not what the products wait for.
 //
-// When there are too few items for the SMs, and a workspace (the paged cache), an item's key tiles are split
-// over several CTAs; each leaves its rows' unnormalised sums, and a second launch joins them.
+// Few items (and a workspace, with the paged cache): items longer than an SM's share of all key tiles
+// are split into parts, which go out like items; each leaves its rows' unnormalised sums, and a second
+// launch joins them.
 //
 // One CTA per SM stays for all its items: the loads, the score products and the search of the next
 // item go on while the softmax warps write the last one's output.  Items go out in the order of their key tiles,
@@ -42,8 +43,9 @@ namespace aexrt {
 constexpr int kTcRows = 128;   // query rows of a tile
 constexpr int kTcKeys = 128;   // keys of a tile
 constexpr int kTcThreads = 384;
-// Key tiles of a part at least: with 2 the joining costs 300 cached keys 22 instead of 19 us, with 8 2000 keys take 33 instead of 28.
-constexpr int kTcMinTiles = 4;
+// Items of fewer key tiles stay whole: below, the joining costs more than the split saves (100 tokens over 300 cached
+// keys: 19 us whole, 22 in parts of 2 tiles).
+constexpr int kTcMinTiles = 6;
 
 // Slots of the K / V ring: what 227 KB hold beside the two Q tiles and the output staging.
 template <int DP>
@@ -113,12 +115,17 @@ struct TcWork {
   int part;        // part of the workspace that the rows go to, -1: the item is whole
 };
 
-// Splitting: the most parts of an item, and where they go.
+// Splitting.  An item of more than T key tiles is split into ceil(tiles / T) parts.  T is a CTA's share of all key tiles,
+// a little more when that leaves one part to a CTA (equal contexts); else, where it does not (ragged ones), two thirds of
+// the share, for parts that even out over the CTAs.  So at most 1.5 * grid items are split, into at most 3 * grid
+// parts.  Items are numbered by falling length, so those that have a part k are the first ones.  The parts go out part 0
+// of every item first, then the parts 1, ...; part k of item r lies at bases[k] + r.
 struct TcSplit {
-  int parts;       // 1: none
-  JoinHead* heads; // [items]
-  float* sums;     // [items][parts][256][head_dim]
-  float* stats;    // [items][parts][256][2]
+  int* split_items; // of the call
+  int* bases;       // [3 * grid]
+  JoinHead* heads;  // [2 * grid]
+  float* sums;      // [3 * grid][256][head_dim]
+  float* stats;     // [3 * grid][256][2]
 };
 
 // Numbers the items of a call: descending in key tiles while a warp can hold every sequence's lengths
@@ -132,6 +139,8 @@ struct TcFinder {
   // of sequence 32 * h + lane: items, len_k - len_q, key tiles of the last item and what that counts for
   int items[kHeld], shift[kHeld], tiles[kHeld], last[kHeld];
   int total = 0, top = 0;  // of all sequences: items, key tiles at most
+  int64_t volume = 0;      // items times their sequence's most key tiles
+  int level = 0;           // of the item found last
   int base = 0;            // by sequence: the first sequence of the 32 looked at, and the items before it
   int64_t before = 0;
 
@@ -154,10 +163,13 @@ struct TcFinder {
           }
         }
         total += items[h];
+        volume += static_cast<int64_t>(items[h]) * tiles[h];
         top = max(top, tiles[h]);
       }
       total = __reduce_add_sync(~0u, total);
       top = __reduce_max_sync(~0u, top);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) volume += __shfl_xor_sync(~0u, volume, o);
     }
   }
   __device__ __forceinline__ int rows_of(int s) const { return kPaged ? min(q_len(p, s), p.max_q) : q_len(p, s); }
@@ -171,8 +183,8 @@ struct TcFinder {
     const int e = (level - 1) * kTcKeys + 1 - shift[h];
     if (e <= 0) return before_last;
     int few = static_cast<int>(static_cast<float>(e - 1) * per_token);  // floor((e - 1) / tokens), then made exact
-    while (few * static_cast<int64_t>(tokens) > e - 1) --few;
-    while ((few + 1) * static_cast<int64_t>(tokens) <= e - 1) ++few;
+    while (few * tokens > e - 1) --few;
+    while ((few + 1) * tokens <= e - 1) ++few;
     return max(0, before_last - few);
   }
   __device__ __forceinline__ int all_from(int level) const {
@@ -180,6 +192,14 @@ struct TcFinder {
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
       if (32 * h < p.num_seqs) n += items_from(h, level) + (last[h] >= max(level, 0) ? 1 : 0);
+    return __reduce_add_sync(~0u, n);
+  }
+  // Parts of at most `size` key tiles that all items make, each counted like its sequence's longest.
+  __device__ __forceinline__ int64_t parts_at_most(int size) const {
+    int n = 0;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+      if (32 * h < p.num_seqs) n += items[h] * ((tiles[h] + size - 1) / size);  // items of a split call: 1.5 for an SM at most
     return __reduce_add_sync(~0u, n);
   }
   __device__ __forceinline__ void fill(TcWork& w, int s, int tile) const {
@@ -200,6 +220,7 @@ struct TcFinder {
         const int mid = (lo + hi + 1) >> 1;
         if (all_from(mid) > item) lo = mid; else hi = mid - 1;
       }
+      level = lo;
       int rank = static_cast<int>(item) - all_from(lo + 1);  // among the items of exactly this level
 #pragma unroll
       for (int h = 0; h < kHeld; ++h) {
@@ -345,38 +366,63 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 10) {
       // ---------------------------------------------------------------- items
       TcFinder<kPaged> finder(p, 2 * tokens);
+      // splitting, when the finder numbers by length: key tiles of a part, and parts of the longest item
+      const int64_t all = static_cast<int64_t>(finder.total) * p.kv_heads;
+      const bool splits = kSplit && finder.total > 0;
+      int size = 1, most = 1;
+      // items and heads with a part k, of those that are split
+      auto with_part = [&](int k) { return finder.all_from(max(1, k) * size + 1) * p.kv_heads; };
+      if (splits) {
+        const int grid = gridDim.x;
+        const int share = max(kTcMinTiles, static_cast<int>((finder.volume * p.kv_heads + grid - 1) / grid));
+        bool fits = false;
+        for (size = share; all <= grid && 10 * size <= 13 * share; size += max(1, size / 16))
+          if ((fits = finder.parts_at_most(size) * p.kv_heads <= grid)) break;
+        if (!fits) size = max(kTcMinTiles, (2 * share + 2) / 3);
+        most = max(1, (finder.top + size - 1) / size);
+      }
+      const int first = splits && most > 1 ? with_part(0) : 0;  // the items that are split
+      int part = 0;             // of the numbers that are handed out now, their first, and how many there are
+      int64_t part_start = 0, part_count = all;
       for (int k = 0;; ++k) {
-        const int64_t number = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        const int64_t rest = number / p.kv_heads, number_of = kSplit ? rest / split.parts : rest;
+        int64_t number = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (splits) {
+          while (number >= part_start + part_count && part + 1 < most) {
+            part_start += part_count;
+            part_count = with_part(++part);
+          }
+          number -= part_start;
+        }
         TcWork w = {};
         w.end = INT_MAX;
         w.part = -1;
-        bool found = finder.find(number_of, w);
-        w.head = static_cast<int>(number % p.kv_heads);
-        if constexpr (kSplit) {  // one number per CTA
-          const int part = static_cast<int>(rest % split.parts);
-          const int64_t slot = number_of * p.kv_heads + w.head;
-          JoinHead head = {};
-          if (found) {
-            const TcTiles<kSplit> t(p, w, tokens);
-            const int parts = clampi(t.nmax / kTcMinTiles, 1, split.parts);
-            if (parts > 1) {
-              head = JoinHead{parts, t.valid[0] + t.valid[1], w.q0 + t.first[0], w.head};
-              w.begin = static_cast<int>(static_cast<int64_t>(t.nmax) * part / parts);
-              w.end = static_cast<int>(static_cast<int64_t>(t.nmax) * (part + 1) / parts);
-              w.part = static_cast<int>(slot * split.parts + part);
-            }
-            found = part < parts;
+        const bool found = (!splits || number < part_count) && finder.find(number / p.kv_heads, w);
+        w.head = found ? static_cast<int>(number % p.kv_heads) : -1;
+        if (splits && found) {
+          const int parts = (finder.level + size - 1) / size;
+          if (parts > 1) {
+            const TcTiles<false> t(p, w, tokens);
+            if (part == 0 && lane == 0)
+              split.heads[number] = JoinHead{parts, t.valid[0] + t.valid[1], w.q0 + t.first[0], w.head};
+            w.begin = static_cast<int>(static_cast<int64_t>(t.nmax) * part / parts);
+            w.end = static_cast<int>(static_cast<int64_t>(t.nmax) * (part + 1) / parts);
+            w.part = static_cast<int>(number + (part ? first + part_start - all : 0));
           }
-          if (part == 0 && lane == 0 && slot * split.parts < gridDim.x) split.heads[slot] = head;
         }
-        if (!found) w.head = -1;
         if (!__all_sync(~0u, wait(w_empty + (k & 1), (k >> 1) + 1))) break;
         if (lane == 0) {
           work[k & 1] = w;
           mbar_arrive(w_full + (k & 1));
         }
         if (!found) break;
+      }
+      if (kSplit && blockIdx.x == 0) {  // for the joining
+        int base = 0;
+        for (int k = 0; k < most && first; ++k) {
+          if (lane == 0) split.bases[k] = base;
+          base += with_part(k);
+        }
+        if (lane == 0) *split.split_items = first;
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------------- loads
@@ -460,27 +506,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tma_load_4d(smem + L::kQ + s * L::kTile + h * 16384, &q_map, q_full + s, h * 64, 0, w.head, w.q0 + t.first[s]);
           }
         };
+        // The page of this lane's box of key tile j (outside the cache for what lies behind the last key: zeros)
+        const int box_rows = kPaged ? min(1 << p.page_shift, kTcKeys) : kTcKeys;
+        auto page_of = [&](int j) {
+          const int key = j * kTcKeys + lane * box_rows;
+          if (!kPaged || lane * box_rows >= kTcKeys || key >= t.key_end) return p.kv_tokens;
+          const int id = __ldg(p.block_table + w.seq * p.table_stride + (key >> p.page_shift));
+          if (id >= 0 && id < p.kv_tokens) return id;
+          atomicOr(p.status, kAttnBadPage);
+          return p.kv_tokens;
+        };
         // one K or V tile; the bytes count whole boxes, what lies outside the tensor arrives as zeros
-        auto load_kv = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j) {
+        auto load_kv = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j, int page) {
           if (lane == 0) mbar_arrive_expect_tx(bar, L::kTile);
           __syncwarp();
           if constexpr (kPaged) {
-            const int rows = min(1 << p.page_shift, kTcKeys);
-            const int key = j * kTcKeys + lane * rows;
-            if (lane * rows < kTcKeys) {
-              int page = p.kv_tokens;  // outside: zeros
-              if (key < t.key_end) {
-                const int id = __ldg(p.block_table + w.seq * p.table_stride + (key >> p.page_shift));
-                if (id >= 0 && id < p.kv_tokens) page = id; else atomicOr(p.status, kAttnBadPage);
-              }
+            if (lane * box_rows < kTcKeys) {
+              const int row = (j * kTcKeys + lane * box_rows) & ((1 << p.page_shift) - 1);
               for (int h = 0; h < kHalves; ++h)
-                tma_load_4d(dst + h * 16384 + lane * rows * 128, map, bar, h * 64, w.head, key & ((1 << p.page_shift) - 1), page);
+                tma_load_4d(dst + h * 16384 + lane * box_rows * 128, map, bar, h * 64, w.head, row, page);
             }
           } else if (lane == 0) {
             for (int h = 0; h < kHalves; ++h) tma_load_3d(dst + h * 16384, map, bar, h * 64, w.head, w.k0 + j * kTcKeys);
           }
           __syncwarp();
         };
+        // pages of the key tiles of the V before last K, of the last K, and of the next one, looked up a tile ahead
+        int page_v = 0, page_k = 0, page_next = t.nmax ? page_of(kSplit ? w.begin : 0) : 0;
         bool released = false;
         load_q(0);
         for (int i = 0; i < 2 * t.nmax && ok; ++i, ++it) {  // K0 K1 V0 K2 V1 ... as the products take them
@@ -490,7 +542,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const bool dirty = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
           ok = wait_serving(kv_empty + slot, it / NS + 1);
           if (!ok) break;
-          load_kv(is_v ? &v_map : &k_map, smem + L::kRing + slot * L::kTile, dirty ? raw + slot : kv_full + slot, j);
+          if (!is_v) {
+            page_v = page_k;
+            page_k = page_next;
+          }
+          load_kv(is_v ? &v_map : &k_map, smem + L::kRing + slot * L::kTile, dirty ? raw + slot : kv_full + slot, j,
+                  is_v && i + 1 < 2 * t.nmax ? page_v : page_k);
+          if (kPaged && !is_v) page_next = page_of(j + 1);
           if (i == 0) load_q(1);
           if (dirty) {
             const int to = min(last, kTcKeys);
@@ -809,15 +867,17 @@ template <typename T>
 __global__ void __launch_bounds__(kTcJoinThreads) attention_tc_join_kernel(const AttnParams p, const TcSplit split) {
   grid_dep_launch();
   grid_dep_wait();
-  const JoinHead item = split.heads[blockIdx.x];
-  if (item.parts == 0) return;
-  const int tokens = kTcRows / p.group, vecs = p.head_dim / 8;
-  for (int i = threadIdx.x; i < kTcJoinRows * vecs; i += kTcJoinThreads) {
-    const int r = blockIdx.y * kTcJoinRows + i / vecs, in_tile = r & 127, row_token = in_tile / p.group;
-    const int token = (r >> 7) * tokens + row_token;
-    if (row_token >= tokens || token >= item.rows) continue;
-    auto row_of = [&](int k) { return (static_cast<int64_t>(blockIdx.x) * split.parts + k) * 256 + r; };
-    join_row<T>(p, split.sums, split.stats, item.parts, row_of, i % vecs * 8, item.q0 + token, item.head * p.group + in_tile % p.group);
+  const int tokens = kTcRows / p.group, vecs = p.head_dim / 8, items = *split.split_items;
+  for (int n = blockIdx.x; n < items; n += gridDim.x) {
+    const JoinHead item = split.heads[n];
+    for (int i = threadIdx.x; i < kTcJoinRows * vecs; i += kTcJoinThreads) {
+      const int r = blockIdx.y * kTcJoinRows + i / vecs, in_tile = r & 127, row_token = in_tile / p.group;
+      const int token = (r >> 7) * tokens + row_token;
+      if (row_token >= tokens || token >= item.rows) continue;
+      auto row_of = [&](int k) { return (static_cast<int64_t>(split.bases[k]) + n) * 256 + r; };
+      join_row<T>(p, split.sums, split.stats, item.parts, row_of, i % vecs * 8, item.q0 + token,
+                  item.head * p.group + in_tile % p.group);
+    }
   }
 }
 
