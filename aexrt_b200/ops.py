@@ -491,6 +491,8 @@ def attention_paged_workspace(q, k_cache, num_seqs: int, max_q: int):
     what, torch = "attention_paged", _torch()
     (tokens, heads, dim), qs = _heads(q, what, "q", 3)
     k_shape, ks = _heads(k_cache, what, "k_cache", 4)
+    if max_q < 0:
+        raise ValueError(f"{what}: max_q must not be negative")
     desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1, 1.0, k_shape[0],
                       k_shape[1], 0, 0, qs[0], qs[1], heads * dim, dim, ks[1], ks[2], ks[0], ks[1], ks[2], ks[0])
     n = _call(lambda desc, stream: _native.load().aexrt_b200_attention_paged_workspace(desc), what, torch, (q, k_cache), 0, (desc,))
@@ -515,9 +517,13 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
     if k_shape != v_shape or k_shape[3] != dim or not q.dtype is k_cache.dtype is v_cache.dtype:
         raise ValueError(f"{what}: the caches must have one shape, and q's type and head size")
     num_seqs = kv_lens.shape[0]
+    if max_q < 0:
+        raise ValueError(f"{what}: max_q must not be negative")
     table, columns, table_stride = _table(block_table, what, num_seqs, torch.int32)
     if workspace is None:
         workspace = attention_paged_workspace(q, k_cache, num_seqs, max_q)
+        if stream is not None and workspace.numel():  # not reused before that stream has passed the call
+            workspace.record_stream(torch.cuda.ExternalStream(_stream(stream), device=q.device))
     elif not workspace.is_contiguous():
         raise ValueError(f"{what}: workspace must be contiguous")
     desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1 if causal else 0,

@@ -461,7 +461,9 @@ int aexrt_b200_act_quantize_f16_noalloc(const void* x, uint32_t n, uint32_t c, u
  *     lengths are cut to the tensors' extents: nothing outside them is read or written.  Rows of
  *     q behind the last sequence are not read, and their rows of out and lse are left as they were.
  *   - Nothing that a row does not see reaches its output, NaN and infinities in masked places,
- *     in unused cache rows and in neighbouring sequences included.
+ *     in unused cache rows and in neighbouring sequences included.  Infinite and NaN values that a
+ *     row sees make its outputs infinite or NaN (an infinity whose probability rounds to 0 gives NaN); a NaN
+ *     or +inf score makes its row NaN.
  *   - head_dim: a multiple of 8 from 8 to 128; q_heads / kv_heads: at most 128.  Pointers 16-byte
  *     aligned, strides (elements) multiples of 8, each head's head_dim elements contiguous.
  *     Every offset is computed in 64 bits.

@@ -158,6 +158,8 @@ def test_tensor_wrappers_refuse_bad_shapes():
         ops.attention_paged(q, k, k, cu[None], cu, cu, 1)
     with pytest.raises(ValueError, match="CUDA"):
         ops.page_tables(cu, cu, torch.zeros(2, 3, dtype=torch.int32), cu, cu, 16, max_tokens=4)
+    with pytest.raises(ValueError, match="max_q"):
+        ops.attention_paged(q, torch.zeros(2, 16, 2, 64, dtype=h), torch.zeros(2, 16, 2, 64, dtype=h), cu[None], cu, cu[:1], -1)
     with pytest.raises(ValueError, match="max_tokens"):
         ops.page_tables(cu, cu, torch.zeros(2, 3, dtype=torch.int32), cu, cu, 16)
     with pytest.raises(ValueError, match="one type"):

@@ -694,6 +694,79 @@ def test_on_another_stream_and_side_by_side():
         oracle.check(o[0], o[1], *x[6])
 
 
+@pytest.mark.parametrize("new", [1, 90])
+def test_workspaces_allocated_for_another_stream_are_kept_until_it_is_done(new):
+    """Calls on a side stream that allocate their own workspaces, with other work on the current stream that would reuse
+    their memory at once."""
+    g = generator(33)
+    kv = [6000, 4000 + new]
+    kc, vc, table, ks, vs = cache_of(g, kv, 16, 2, 128, BF16)
+    q = rand(g, 2 * new, 8, 128, dtype=BF16)
+    cu, lens = ints([0, new, 2 * new]), ints(kv)
+    want = expect(q, ks, vs, [new] * 2, 128 ** -0.5, True)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = [torch.empty_like(q) for _ in range(8)]
+    for o in outs:
+        ops.attention_paged(q, kc, vc, table, cu, lens, new, out=o, stream=side)
+        size = ops.attention_paged_workspace(q, kc, 2, new).numel()
+        torch.full((max(1, size // 4),), math.nan, device="cuda")
+    torch.cuda.synchronize()
+    for o in outs:
+        oracle.check(o, None, *want)
+
+
+def test_two_captured_graphs_share_a_workspace_in_turn():
+    g = generator(34)
+    sets, graphs = [], []
+    for kv in ([5000, 70], [33, 2100]):
+        kc, vc, table, ks, vs = cache_of(g, kv, 16, 2, 64, F16)
+        q = rand(g, 2, 8, 64, dtype=F16)
+        sets.append([q, kc, vc, table, ints([0, 1, 2]), ints(kv), expect(q, ks, vs, [1, 1], 0.125, True), torch.empty_like(q)])
+    ws = ops.attention_paged_workspace(sets[0][0], sets[0][1], 2, 1)
+    for x in sets:
+        ops.attention_paged(*x[:6], 1, out=x[7], workspace=ws)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ops.attention_paged(*x[:6], 1, out=x[7], workspace=ws)
+    for _ in range(3):
+        for gr, x in zip(graphs, sets):
+            x[7].fill_(5.0)
+            ws.random_()
+            gr.replay()
+            oracle.check(x[7], None, *x[6])
+
+
+def test_broadcast_heads():
+    """k and v of one head expanded over several (stride 0): the result of a real copy, or a refusal."""
+    g = generator(35)
+    q = rand(g, 70, 4, 64, dtype=F16)
+    k, v = (rand(g, 70, 1, 64, dtype=F16) for _ in range(2))
+    cu = ints([0, 70])
+    want = ops.attention_packed(q, k.expand(70, 4, 64).contiguous(), v.expand(70, 4, 64).contiguous(), cu, cu)
+    try:
+        out = ops.attention_packed(q, k.expand(70, 4, 64), v.expand(70, 4, 64), cu, cu)
+    except _native.AexrtError:
+        return
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("ctx,new,heads", [([30000], 70, (8, 2)), ([20000, 300, 9000], 65, (4, 4)), ([50, 12000, 700, 0, 3000], 33, (8, 2)),
+                                           ([9000], 300, (4, 1)), ([15000] * 3, 80, (2, 1)), ([700], 65, (4, 4))])
+def test_paged_split_over_long_contexts(ctx, new, heads):
+    """Few items over long and ragged contexts: the key ranges of an item go to several blocks."""
+    g = generator(36)
+    hq, hk = heads
+    kv = [c + new for c in ctx]
+    kc, vc, table, ks, vs = cache_of(g, kv, 16, hk, 128, BF16, poison=math.nan)
+    q = rand(g, new * len(ctx), hq, 128, dtype=BF16, std=2.0)
+    cu = ints(oracle.sums([new] * len(ctx)))
+    for causal in (True, False):
+        out, lse = ops.attention_paged(q, kc, vc, table, cu, ints(kv), new, causal=causal, return_lse=True)
+        no_status()
+        oracle.check(out, lse, *expect(q, ks, vs, [new] * len(ctx), 128 ** -0.5, causal))
+
+
 def test_with_programmatic_launches():
     """The library's programmatic launch flag: kernels that follow one another still see each other's writes."""
     lib = _native.load()
