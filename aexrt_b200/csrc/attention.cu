@@ -99,6 +99,18 @@ bool strides_ok(const char* what, uint64_t a, uint64_t b, uint64_t c = 0) {
   return true;
 }
 
+// The description with the strides of dimensions of one element, which nothing is addressed by, set to a row.
+AexrtB200AttentionDesc with_used_strides(const AexrtB200AttentionDesc* d, bool paged) {
+  AexrtB200AttentionDesc u = *d;
+  const uint64_t row = std::max(8u, d->head_dim);
+  if (d->q_tokens <= 1) u.q_token_stride = u.out_token_stride = row * std::max(1u, d->q_heads);
+  if (d->q_heads <= 1) u.q_head_stride = u.out_head_stride = row;
+  if (d->kv_heads <= 1) u.k_head_stride = u.v_head_stride = row;
+  if ((paged ? d->page_size : d->kv_tokens) <= 1) u.k_token_stride = u.v_token_stride = row;
+  if (paged && d->kv_tokens <= 1) u.k_page_stride = u.v_page_stride = row;
+  return u;
+}
+
 // The checks that packed and paged attention share (no pointers).
 bool desc_ok(const AexrtB200AttentionDesc* d, bool paged) {
   const char* what = paged ? "attention_paged" : "attention_packed";
@@ -319,6 +331,9 @@ int launch_tc(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, 
 
 int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, const void* k, const void* v,
                                 const int32_t* cu_q, const int32_t* cu_k, void* out, float* lse, void* stream) {
+  if (!d || d->struct_size != sizeof(AexrtB200AttentionDesc)) return desc_ok(d, false) ? 1 : 0;
+  const AexrtB200AttentionDesc used = with_used_strides(d, false);
+  d = &used;
   if (!desc_ok(d, false)) return 0;
   if (d->q_tokens == 0 || d->num_seqs == 0) return 1;
   if (!q || !cu_q || !cu_k || !out || (d->kv_tokens && (!k || !v))) return fail("attention_packed: null pointer");
@@ -333,6 +348,9 @@ int aexrt_b200_attention_packed(const AexrtB200AttentionDesc* d, const void* q, 
 }
 
 uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* d) {
+  if (!d || d->struct_size != sizeof(AexrtB200AttentionDesc)) return desc_ok(d, true), ~0ull;
+  const AexrtB200AttentionDesc used = with_used_strides(d, true);
+  d = &used;
   if (!desc_ok(d, true)) return ~0ull;
   if (d->q_tokens == 0 || d->num_seqs == 0 || d->max_q == 0) return 0;
   const uint32_t rows = few_rows(d);
@@ -342,6 +360,9 @@ uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* d) {
 int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, const void* k_cache, const void* v_cache,
                                const int32_t* block_table, const int32_t* cu_q, const int32_t* kv_lens, void* out,
                                float* lse, void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (!d || d->struct_size != sizeof(AexrtB200AttentionDesc)) return desc_ok(d, true) ? 1 : 0;
+  const AexrtB200AttentionDesc used = with_used_strides(d, true);
+  d = &used;
   if (!desc_ok(d, true)) return 0;
   if (d->q_tokens == 0 || d->num_seqs == 0 || d->max_q == 0) return 1;
   if (!q || !cu_q || !kv_lens || !out || (d->kv_tokens && (!k_cache || !v_cache)) || (d->table_columns && !block_table))
@@ -404,9 +425,13 @@ int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uin
   if (!raise_smem(reinterpret_cast<const void*>(page_tables_kernel),
                   (3 * kTablesMaxSeqs + 2) * static_cast<int>(sizeof(int32_t))))
     return 0;
-  const unsigned ctas = std::min<unsigned>(kTablesMaxCtas, std::max<unsigned>(1, (slot_capacity + 1023) / 1024));
+  // In place, every block has to have read the lengths and the state before one writes them: one cluster.  Otherwise the
+  // blocks need nothing of one another.
+  const bool in_place = kv_lens == ctx_lens || free_state_out == free_state_in;
+  const unsigned most = in_place ? kTablesMaxCtas : static_cast<unsigned>(sm_count());
+  const unsigned ctas = std::min(most, std::max(1u, (slot_capacity + kTablesThreads - 1) / kTablesThreads));
   return cuda_ok(launch_kernel_cluster(page_tables_kernel, dim3(ctas), dim3(kTablesThreads), smem,
-                                       static_cast<cudaStream_t>(stream), ctas, p),
+                                       static_cast<cudaStream_t>(stream), in_place ? ctas : 1, p),
                  "page_tables launch")
              ? 1
              : 0;
@@ -421,6 +446,11 @@ int aexrt_b200_kv_append(const void* k, const void* v, uint32_t tokens, uint32_t
   if (head_dim == 0 || head_dim % 8 || head_dim > 65536) return fail("kv_append: head_dim must be a multiple of 8");
   if (kv_heads == 0 || kv_heads > 65535u) return fail("kv_append: kv_heads must be from 1 to 65535");
   if (tokens > (1u << 30)) return fail("kv_append: at most 2^30 tokens");
+  // dimensions of one element: nothing is addressed by their strides
+  if (tokens <= 1) k_token_stride = v_token_stride = head_dim;
+  if (kv_heads <= 1) k_head_stride = v_head_stride = k_cache_head_stride = v_cache_head_stride = head_dim;
+  if (page_size <= 1) k_cache_token_stride = v_cache_token_stride = head_dim;
+  if (num_pages <= 1) k_cache_page_stride = v_cache_page_stride = head_dim;
   if (page_size == 0 || page_size > 1024 || (page_size & (page_size - 1)))
     return fail("kv_append: page_size must be a power of two up to 1024");
   if (static_cast<uint64_t>(num_pages) * page_size >= (1ull << 31)) return fail("kv_append: the cache has 2^31 slots or more");

@@ -51,7 +51,7 @@ __device__ __forceinline__ int find_request(const int32_t* sums, int n, int x) {
   return lo;
 }
 
-// One thread-block cluster.  Every CTA sums all requests' new tokens and new pages into its own shared
+// Every CTA sums all requests' new tokens and new pages into its own shared
 // memory (a few KB, read from L2 by each), then fills its share of the slots, of the new table
 // columns and of the per-request outputs.  A slot in a new page takes the page from the free stack
 // directly, by the page's rank in the order of taking, so no CTA waits for another's table writes;
@@ -94,7 +94,9 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
   const int top = min(max(0, __ldcg(p.state_in)), p.free_capacity);
   if (n == 0 && threadIdx.x == 0) cu[0] = taken[0] = 0;
   __syncthreads();
-  cluster_sync_all();  // every CTA has read ctx and the state: outputs may take their place
+  // in place, the CTAs are one cluster: every one has read ctx and the state, outputs may take their place
+  // (alone, each is a cluster of its own)
+  cluster_sync_all();
   const int at = blockIdx.x * kTablesThreads + threadIdx.x, step = gridDim.x * kTablesThreads;
   for (int i = at; i <= n; i += step) {
     p.cu_q[i] = cu[i];

@@ -403,16 +403,13 @@ def _dtype16(t, what: str, torch) -> int:
 
 
 def _heads(t, what: str, name: str, dims: int):
-    """Shape and strides of a [..., heads, head_dim] tensor with contiguous heads.  A dimension of size 1, whose stride
-    torch leaves arbitrary, counts one row."""
+    """Shape and strides of a [..., heads, head_dim] tensor with contiguous heads (the library ignores the stride of a
+    dimension of size 1, which torch leaves arbitrary)."""
     shape, strides = t.shape, t.stride()
     if len(shape) != dims:
         raise ValueError(f"{what}: {name} must have {dims} dimensions")
     if strides[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what}: each head of {name} must be contiguous")
-    if 1 in shape:
-        row = max(8, shape[-1])
-        strides = tuple(row if n == 1 else s for n, s in zip(shape, strides))
     return shape, strides
 
 
@@ -445,17 +442,19 @@ def _call(fn, what: str, torch, tensors, stream, args):
     return fn(*args, handle)
 
 
-def _outputs(what: str, torch, q, out, lse, return_lse):
+def _outputs(what: str, torch, q, q_shape, out, lse, return_lse):
+    """The outputs given or made: (out, its strides, lse)."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype:
+        out = torch.empty(q_shape, dtype=q.dtype, device=q.device)
+    shape, strides = _heads(out, what, "out", 3)
+    if shape != q_shape or out.dtype is not q.dtype:
         raise ValueError(f"{what}: out must have q's shape and type")
     if lse is None:
         if return_lse:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    elif lse.shape != q.shape[:2] or lse.dtype is not torch.float32 or not lse.is_contiguous():
+            lse = torch.empty(q_shape[:2], dtype=torch.float32, device=q.device)
+    elif lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape != q_shape[:2] or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor [tokens, heads]")
-    return out, lse
+    return out, strides, lse
 
 
 def attention_packed(q, k, v, cu_q, cu_k, causal: bool = True, scale: Optional[float] = None, out=None, lse=None,
@@ -466,11 +465,11 @@ def attention_packed(q, k, v, cu_q, cu_k, causal: bool = True, scale: Optional[f
     sequence.  ``scale`` defaults to d ** -0.5.  Returns out, or (out, lse) with ``return_lse`` or a
     given ``lse`` (fp32 [q_tokens, q_heads], natural logarithm).  Rows behind the last sequence are left as they were."""
     what, torch = "attention_packed", _torch()
-    (tokens, heads, dim), qs = _heads(q, what, "q", 3)
+    q_shape, qs = _heads(q, what, "q", 3)
+    tokens, heads, dim = q_shape
     k_shape, ks = _heads(k, what, "k", 3)
     v_shape, vs = _heads(v, what, "v", 3)
-    out, lse = _outputs(what, torch, q, out, lse, return_lse)
-    _, os_ = _heads(out, what, "out", 3)
+    out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse)
     if k_shape != v_shape or k_shape[2] != dim or not q.dtype is k.dtype is v.dtype:
         raise ValueError(f"{what}: k and v must have one shape, and q's type and head size")
     num_seqs = cu_q.shape[0] - 1
@@ -509,11 +508,11 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
     of each sequence, the new tokens' own among them (see :func:`page_tables` and :func:`kv_append`).  ``workspace``:
     from :func:`attention_paged_workspace`; without one the call allocates it."""
     what, torch = "attention_paged", _torch()
-    (tokens, heads, dim), qs = _heads(q, what, "q", 3)
+    q_shape, qs = _heads(q, what, "q", 3)
+    tokens, heads, dim = q_shape
     k_shape, ks = _heads(k_cache, what, "k_cache", 4)
     v_shape, vs = _heads(v_cache, what, "v_cache", 4)
-    out, lse = _outputs(what, torch, q, out, lse, return_lse)
-    _, os_ = _heads(out, what, "out", 3)
+    out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse)
     if k_shape != v_shape or k_shape[3] != dim or not q.dtype is k_cache.dtype is v_cache.dtype:
         raise ValueError(f"{what}: the caches must have one shape, and q's type and head size")
     num_seqs = kv_lens.shape[0]

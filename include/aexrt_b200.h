@@ -465,7 +465,8 @@ int aexrt_b200_act_quantize_f16_noalloc(const void* x, uint32_t n, uint32_t c, u
  *     row sees make its outputs infinite or NaN (an infinity whose probability rounds to 0 gives NaN); a NaN
  *     or +inf score makes its row NaN.
  *   - head_dim: a multiple of 8 from 8 to 128; q_heads / kv_heads: at most 128.  Pointers 16-byte
- *     aligned, strides (elements) multiples of 8, each head's head_dim elements contiguous.
+ *     aligned, strides (elements) multiples of 8 (that of a dimension of size 1 is ignored), each
+ *     head's head_dim elements contiguous.
  *     Every offset is computed in 64 bits.
  *   - Launches are asynchronous on `stream` and allocate nothing. */
 #define AEXRT_B200_DTYPE_F16 0u
