@@ -33,6 +33,11 @@
 // loads, warp 10 finds the items.  Registers are split by warpgroup, 216 for a softmax thread (it
 // holds a whole row of S) and 72 for the others, 2 * 216 + 72 = 3 * 168 as launched.
 // TMEM columns: S 0-127, P0 128-191, P1 192-255, O0 256-, O1 384-.
+//
+// Measured (32 heads over 8, head size 128, bf16, 1000 W limit): one prompt of 16384 tokens 1.69 ms (1305 TFLOP/s) at
+// first, 1.94 ms in long runs at 1.55 GHz; 19 ragged prompts of 15001 tokens 228 us; 2 x 1024 tokens over 32768 cached keys
+// 480 us.  In long prompts the tensor pipe is 64 % active; ragged ones lose 9000 clocks an item to the last product's
+// latency and the output, which warps of their own did not win back (registers: 176 / 80 / 80; 260 -> 285 us).
 #pragma once
 #include <climits>
 

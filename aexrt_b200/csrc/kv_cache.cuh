@@ -56,7 +56,8 @@ __device__ __forceinline__ int find_request(const int32_t* sums, int n, int x) {
 // columns and of the per-request outputs.  A slot in a new page takes the page from the free stack
 // directly, by the page's rank in the order of taking, so no CTA waits for another's table writes;
 // the cluster barrier between the reads of lengths and state and all writes is what lets kv_lens
-// and the state be updated in place.  Latency-bound: a few dependent rounds of loads and one barrier.
+// and the state be updated in place.  Latency-bound: a few dependent rounds of loads and one barrier
+// (256 requests of one token: 5.8 us; 65536 new tokens, on 64 blocks: 10 us, a binary search per slot).
 __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const TablesParams p) {
   extern __shared__ int32_t sums[];  // new tokens [n + 1], new pages [n + 1], context [n]
   grid_dep_launch();
@@ -142,7 +143,8 @@ struct AppendParams {
   int64_t k_ts, k_hs, v_ts, v_hs, kc_ps, kc_ts, kc_hs, vc_ps, vc_ts, vc_hs;  // in 16-byte pieces
 };
 
-// One thread copies one 16-byte piece of k and the same piece of v.
+// One thread copies one 16-byte piece of k and the same piece of v: HBM-bound, 32768 rows of 8 heads of 128 in
+// 45 us (5.96 TB/s); 64 rows in 2 us.
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
   grid_dep_launch();
   grid_dep_wait();
