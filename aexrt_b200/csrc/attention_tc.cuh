@@ -30,13 +30,13 @@
 // Roles: warps 0-3 softmax of tile 0, warps 4-7 of tile 1, one thread each of warps 8 and 11 issues
 // the MMAs of tile 0 and of tile 1 (one thread for both spent 93 clocks an MMA instead of the
 // pipe's 64: it holds few MMAs, and ran dry whenever the thread looked at its barriers), warp 9
-// loads, warp 10 finds the items.  Registers are split by warpgroup, 216 for a softmax thread (it
+// loads, warp 10 finds the items and cleans V tiles.  Registers are split by warpgroup, 216 for a softmax thread (it
 // holds a whole row of S) and 72 for the others, 2 * 216 + 72 = 3 * 168 as launched.
 // TMEM columns: S 0-127, P0 128-191, P1 192-255, O0 256-, O1 384-.
 //
 // Measured (32 heads over 8, head size 128, bf16, 1000 W limit): one prompt of 16384 tokens 1.69 ms (1305 TFLOP/s) at
-// first, 1.94 ms in long runs at 1.55 GHz; 19 ragged prompts of 15001 tokens 228 us; 2 x 1024 tokens over 32768 cached keys
-// 480 us.  In long prompts the tensor pipe is 64 % active; ragged ones lose 9000 clocks an item to the last product's
+// first, 1.90 ms in long runs at 1.55 GHz; 19 ragged prompts of 15001 tokens 211 us; 2 x 1024 tokens over 32768 cached keys
+// 473 us.  In long prompts the tensor pipe is 64 % active; ragged ones lose 9000 clocks an item to the last product's
 // latency and the output, which warps of their own did not win back (registers: 176 / 80 / 80; 260 -> 285 us).
 #pragma once
 #include <climits>
@@ -278,6 +278,7 @@ template <bool kSplit>
 struct TcTiles {
   int first[2], valid[2], keys[2], n[2];
   int key_end, nmax, common;  // keys at and above `common` are seen by some rows and not by others
+  int unclean;                // from this one on (of all of the item's) V tiles are cleaned before their product
   __device__ __forceinline__ TcTiles(const AttnParams& p, const TcWork& w, int tokens) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -290,6 +291,7 @@ struct TcTiles {
     key_end = max(keys[0], keys[1]);
     nmax = max(n[0], n[1]);
     common = min(keys_seen(first[0], w.len_q, w.len_k, p.causal), key_end);
+    unclean = (common < key_end ? common : key_end) / kTcKeys;  // a whole last tile that all rows see: none
   }
 };
 
@@ -321,9 +323,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* fixed = reinterpret_cast<int*>(tmem_slot + 1);  // [2]
   TcWork* work = reinterpret_cast<TcWork*>(fixed + 3);  // [2]
-  int4* unclean = reinterpret_cast<int4*>((reinterpret_cast<uintptr_t>(work + 2) + 15) & ~uintptr_t{15});  // [NS], see the loads
   int* fix = reinterpret_cast<int*>(smem + L::kFix);    // [2][kFixInts]
-  static_assert((14 + 3 * tc_slots<DP>() + 4) * 8 + 16 + 2 * sizeof(TcWork) + 16 * tc_slots<DP>() <= 640, "barriers and items fit");
+  static_assert((14 + 3 * tc_slots<DP>() + 4) * 8 + 16 + 2 * sizeof(TcWork) <= 640, "barriers and items fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dep_launch();
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(p_full + i, 128);
       mbar_init(o_done + i, 1);
       mbar_init(w_full + i, 1);
-      mbar_init(w_empty + i, 11);  // the loading warp, two MMA threads, eight softmax warps
+      mbar_init(w_empty + i, 12);  // the loading and the cleaning warp, two MMA threads, eight softmax warps
       mbar_init(s_free + i, 128);
       mbar_init(drain + i, 1);
       fixed[i] = 0;
@@ -389,7 +390,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int first = splits && most > 1 ? with_part(0) : 0;  // the items that are split
       int part = 0;             // of the numbers that are handed out now, their first, and how many there are
       int64_t part_start = 0, part_count = all;
-      for (int k = 0;; ++k) {
+      // Finds item number k of this CTA and puts it out, once every role has left item k - 2.
+      auto publish = [&](int k) {
         int64_t number = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         if (splits) {
           while (number >= part_start + part_count && part + 1 < most) {
@@ -414,12 +416,72 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             w.part = static_cast<int>(number + (part ? first + part_start - all : 0));
           }
         }
-        if (!__all_sync(~0u, wait(w_empty + (k & 1), (k >> 1) + 1))) break;
+        if (!__all_sync(~0u, wait(w_empty + (k & 1), (k >> 1) + 1))) return false;
+        const bool used = fixed[k & 1] != 0;
+        __syncwarp();
+        if (used) {  // by item k - 2
+          for (int i = lane; i < kFixInts; i += 32) fix[(k & 1) * kFixInts + i] = INT_MAX;
+          if (lane == 0) fixed[k & 1] = 0;
+          __syncwarp();
+        }
         if (lane == 0) {
           work[k & 1] = w;
           mbar_arrive(w_full + (k & 1));
         }
-        if (!found) break;
+        __syncwarp();
+        return found;
+      };
+      // V tiles that have to be cleaned before their product.  P is 0 where a row does not see a key, but
+      // 0 * inf and 0 * NaN are not: rows behind the last key become zeros (as far as the product goes, a
+      // quarter of the tile), and non-finite values of keys that only some rows see are taken out and put
+      // back into the outputs of the rows that do.  Such a tile lands on a barrier of its own, and this warp
+      // hands it on.
+      uint32_t raws = 0;  // per slot, the phase of that barrier
+      int it = 0;         // ring items of the items before
+      auto clean = [&](int k, const TcWork& w) {
+        const TcTiles<kSplit> t(p, w, tokens);
+        int* fx = fix + (k & 1) * kFixInts;
+        const int begin = kSplit ? w.begin : 0, sub = lane >> 3, piece = lane & 7;
+        for (int j = max(t.unclean - begin, 0); j < t.nmax; ++j) {
+          const int slot = (it + (j + 1 < t.nmax ? 2 * j + 2 : 2 * t.nmax - 1)) % NS, key = (begin + j) * kTcKeys;
+          if (!__all_sync(~0u, wait(raw + slot, (raws >> slot) & 1))) return false;
+          raws ^= 1u << slot;
+          const int last = min(t.key_end - key, kTcKeys), from = max(0, min(t.common - key, last));
+          for (int h = 0; h < kHalves; ++h) {
+            // 16-byte piece c of row r lies at piece c ^ (r % 8): the 128-byte swizzle
+            uint4* tile = reinterpret_cast<uint4*>(smem + L::kRing + slot * L::kTile + h * 16384) + piece;
+#pragma unroll 4
+            for (int r = last + sub; r < min(kTcKeys, (last + 31) & ~31); r += 4) tile[r * 8] = make_uint4(0, 0, 0, 0);
+            for (int r = from + sub; r < last; r += 32) {
+              uint32_t bits = 0;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {  // rows past the end look at this lane's first row again
+                const uint4 x = tile[(r + 4 * i < last ? r + 4 * i : r) * 8];
+                bits |= non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w);
+              }
+              if (bits) {
+                for (int row = r; row < min(r + 32, last); row += 4)
+                  tile[row * 8] = take_non_finite<T>(tile[row * 8], key + row, h * 64 + (piece ^ (row & 7)) * 8, fx);
+                fixed[k & 1] = 1;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kv_full + slot);
+        }
+        it += 2 * t.nmax;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(w_empty + (k & 1));
+        return true;
+      };
+      // two items are out at a time; an item's tiles are cleaned once the next one is out
+      bool more = publish(0) && publish(1);
+      for (int k = 0;; ++k) {
+        const TcWork w = work[k & 1];
+        __syncwarp();
+        if (w.head < 0 || !clean(k, w)) break;
+        more = more && publish(k + 2);
       }
       if (kSplit && blockIdx.x == 0) {  // for the joining
         int base = 0;
@@ -434,77 +496,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t q_bytes = static_cast<uint32_t>(tokens * p.group * 128 * kHalves);
       bool ok = true;
       int it = 0, qs[2] = {0, 0};
-      // V tiles that have to be cleaned before their product.  P is 0 where a row does not see a key, but
-      // 0 * inf and 0 * NaN are not: rows behind the last key become zeros (as far as the product goes, a
-      // quarter of the tile), and non-finite values of keys that only some rows see are taken out and put
-      // back into the outputs of the rows that do.  Such a tile lands on a barrier of its own and is cleaned
-      // while later loads are already on their way.
-      // Of a slot's tile: x, y the rows that are looked at (from, last), z its first key, w its item, and
-      // whether that has no loads after it (bit 31).  `queue`: slots in order, 4 bits each.
-      uint32_t queue = 0, waiting = 0, raws = 0;  // raws: per slot, the phase of its barrier
-      auto clean = [&]() {
-        const int slot = queue & 15;
-        __syncwarp();
-        const int4 u = unclean[slot];
-        const int from = u.x, last = u.y, of = u.w & 1;
-        uint8_t* dst = smem + L::kRing + slot * L::kTile;
-        int* fx = fix + of * kFixInts;
-        const int sub = lane >> 3, piece = lane & 7;  // 16-byte piece c of row r lies at piece c ^ (r % 8): the 128-byte swizzle
-        for (int h = 0; h < kHalves; ++h) {
-          uint4* tile = reinterpret_cast<uint4*>(dst + h * 16384) + piece;
-#pragma unroll 4
-          for (int r = last + sub; r < min(kTcKeys, (last + 31) & ~31); r += 4) tile[r * 8] = make_uint4(0, 0, 0, 0);
-          for (int r = from + sub; r < last; r += 32) {
-            uint32_t bits = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // rows past the end look at this lane's first row again
-              const uint4 x = tile[(r + 4 * i < last ? r + 4 * i : r) * 8];
-              bits |= non_finite_bits<T>(x.x) | non_finite_bits<T>(x.y) | non_finite_bits<T>(x.z) | non_finite_bits<T>(x.w);
-            }
-            if (bits) {
-              for (int row = r; row < min(r + 32, last); row += 4)
-                tile[row * 8] = take_non_finite<T>(tile[row * 8], u.z + row, h * 64 + (piece ^ (row & 7)) * 8, fx);
-              fixed[of] = 1;
-            }
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(kv_full + slot);
-          if (u.w < 0) mbar_arrive(w_empty + of);
-        }
-        raws ^= 1u << slot;
-        queue >>= 4;
-        --waiting;
-      };
-      auto wait_serving = [&](uint64_t* bar, int phase) {  // a wait that cleans what lands first
-        const long long t0 = clock64();
-        while (waiting) {
-          if (__any_sync(~0u, mbar_test_wait(bar, phase & 1))) return true;
-          const int slot = queue & 15;
-          if (__any_sync(~0u, mbar_test_wait(raw + slot, (raws >> slot) & 1)))
-            clean();
-          else if (__any_sync(~0u, clock64() - t0 > kWaitLimitCycles))
-            break;
-        }
-        return __all_sync(~0u, wait(bar, phase)) != 0;
-      };
       TcWork w;
       for (int k = 0; ok; ++k) {
-        ok = wait_serving(w_full + (k & 1), k >> 1);
+        ok = __all_sync(~0u, wait(w_full + (k & 1), k >> 1));
         w = work[k & 1];
         if (!ok || w.head < 0) break;
         const TcTiles<kSplit> t(p, w, tokens);
-        if (fixed[k & 1]) {  // the roles have left the item that used it last
-          __syncwarp();
-          for (int i = lane; i < kFixInts; i += 32) fix[(k & 1) * kFixInts + i] = INT_MAX;
-          if (lane == 0) fixed[k & 1] = 0;
-          __syncwarp();
-        }
         auto load_q = [&](int s) {
           if (!t.n[s] || !ok) return;
-          ok = wait_serving(q_empty + s, qs[s]++ + 1);
+          ok = __all_sync(~0u, wait(q_empty + s, qs[s]++ + 1));
           if (lane == 0 && ok) {
             mbar_arrive_expect_tx(q_full + s, q_bytes);
             for (int h = 0; h < kHalves; ++h)
@@ -538,14 +538,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         // pages of the key tiles of the V before last K, of the last K, and of the next one, looked up a tile ahead
         int page_v = 0, page_k = 0, page_next = t.nmax ? page_of(kSplit ? w.begin : 0) : 0;
-        bool released = false;
         load_q(0);
         for (int i = 0; i < 2 * t.nmax && ok; ++i, ++it) {  // K0 K1 V0 K2 V1 ... as the products take them
           const bool is_v = i + 1 == 2 * t.nmax || (i > 0 && !(i & 1));
           const int slot = it % NS, j = (kSplit ? w.begin : 0) + (is_v ? (i + 1 == 2 * t.nmax ? t.nmax : i >> 1) - 1 : (i + 1) >> 1);
-          const int last = t.key_end - j * kTcKeys, seen = t.common - j * kTcKeys;  // rows of this tile below them
-          const bool dirty = is_v && (last < kTcKeys || (seen < kTcKeys && seen < last));
-          ok = wait_serving(kv_empty + slot, it / NS + 1);
+          const bool dirty = is_v && j >= t.unclean;
+          ok = __all_sync(~0u, wait(kv_empty + slot, it / NS + 1));
           if (!ok) break;
           if (!is_v) {
             page_v = page_k;
@@ -555,21 +553,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   is_v && i + 1 < 2 * t.nmax ? page_v : page_k);
           if (kPaged && !is_v) page_next = page_of(j + 1);
           if (i == 0) load_q(1);
-          if (dirty) {
-            const int to = min(last, kTcKeys);
-            const bool ends = i + 1 == 2 * t.nmax;
-            if (lane == 0) unclean[slot] = make_int4(max(0, min(seen, to)), to, j * kTcKeys, (k & 1) | (ends ? INT_MIN : 0));
-            queue |= static_cast<uint32_t>(slot) << (4 * waiting++);
-            released = ends;
-          }
         }
         __syncwarp();
-        if (!released && lane == 0) mbar_arrive(w_empty + (k & 1));  // else when its last tile has been cleaned
-      }
-      while (waiting && ok) {
-        const int slot = queue & 15;
-        ok = __all_sync(~0u, wait(raw + slot, (raws >> slot) & 1));
-        if (ok) clean();
+        if (lane == 0) mbar_arrive(w_empty + (k & 1));
       }
       if (!ok) {
         // a wait gave up: the loads in flight still have to land before the CTA may leave
