@@ -8,6 +8,11 @@ namespace aexrt {
 // stay below 2^8, far inside fp16, and most tiles need no rescaling of the accumulators.
 constexpr float kLazyLog2 = 8.f;
 
+// s * c - m * c as one multiply-add carries the rounding of m * c, half a step of its own magnitude: 2^-12 here.
+// Beyond, s - m is taken first (exact for the scores that count), so that scores as large as fp32 holds still
+// give finite probabilities.
+constexpr float kLargeLog2 = 4096.f;
+
 // 2^x on the special-function unit (subnormal results flush to 0).
 __device__ __forceinline__ float exp2_sfu(float x) {
   float y;

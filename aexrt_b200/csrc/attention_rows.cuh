@@ -370,12 +370,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] *= f[e >> 1];
     }
-    const float base[2] = {m[0] == -INFINITY ? 0.f : -m[0] * sl2, m[1] == -INFINITY ? 0.f : -m[1] * sl2};
+    const float m0[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
     for (int n = 0; n < kWarpKeys / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = exp2_sfu(fmaf(s[n][e], sl2, base[e >> 1]));
+        s[n][e] = exp2_sfu((s[n][e] - m0[e >> 1]) * sl2);  // the difference first: finite for any finite scores
         l[e >> 1] += s[n][e];
       }
     // ---- O += P V

@@ -708,7 +708,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_st_wait();
           }
         }
-        const float base = m == -INFINITY ? 0.f : -m * sl2;
+        const float m0 = m == -INFINITY ? 0.f : m;
+        float base = -m0 * sl2;
+        const bool large = fabsf(base) > kLargeLog2;  // row by row: no row's result depends on its neighbours
+        if (__any_sync(~0u, large)) {
+          const float first = large ? m0 : 0.f;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - first);
+          if (large) base = 0.f;
+        }
         const uint64_t base2 = f2_pack(base, base), sl22 = f2_pack(sl2, sl2);
         uint64_t sum[2] = {0, 0};
 #pragma unroll

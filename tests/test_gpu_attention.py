@@ -239,6 +239,30 @@ def test_packed_large_and_rising_scores():
             oracle.check(out, lse, *expect(q, [k], [v], [n], 2.0, causal))
 
 
+@pytest.mark.parametrize("dtype,size", [(F16, 60000.0), (BF16, 1e18), (F16, 300.0)])
+def test_scores_of_any_finite_size(dtype, size):
+    """Equal huge scores give the mean, and one that is larger still takes all: packed, one token and a chunk over a cache."""
+    n, d, page = 300, 64, 16
+    g = generator(37)
+    q = torch.full((n, 2, d), size, dtype=dtype, device="cuda")
+    k = torch.full((n, 2, d), size, dtype=dtype, device="cuda")
+    k[40:, 1] = -k[40:, 1]
+    v = rand(g, n, 2, d, dtype=dtype)
+    cu = ints([0, n])
+    u = oracle.half_step(dtype)
+    kc, vc = (torch.zeros(-(-n // page), page, 2, d, dtype=dtype, device="cuda") for _ in range(2))
+    ops.kv_append(k, v, torch.arange(n, dtype=torch.int32, device="cuda"), kc, vc)
+    table = torch.arange(kc.shape[0], dtype=torch.int32, device="cuda")[None]
+    mean = v.double().cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None, None]
+    mean[40:, 1] = mean[39, 1]  # head 1: the keys from 40 on score far below
+    # probabilities are 1 before normalising, so exact in 16 bits: the output's rounding and fp32 sums of n terms
+    tol = u * mean.abs() + n * 2.0 ** -22 * v.double().abs().max() + 2.0 ** -25
+    for out, rows in ((ops.attention_packed(q, k, v, cu, cu), slice(0, n)),
+                      (ops.attention_paged(q[-1:], kc, vc, table, ints([0, 1]), ints([n]), 1), slice(n - 1, n)),
+                      (ops.attention_paged(q[-80:], kc, vc, table, ints([0, 80]), ints([n]), 80), slice(n - 80, n))):
+        assert bool(((out.double() - mean[rows]).abs() <= tol[rows]).all())
+
+
 def test_packed_large_values_keep_their_range():
     """fp16's largest values: the weighted sum stays within them."""
     g = generator(11)
