@@ -189,7 +189,9 @@ bool kv_maps(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, u
     const void* base = i ? p.v : p.k;
     const uint64_t ts = 2 * (i ? d->v_token_stride : d->k_token_stride), hs = 2 * (i ? d->v_head_stride : d->k_head_stride);
     const uint64_t rows = std::max(1u, d->kv_tokens);
-    if (d->kv_tokens == 0) base = p.q;  // no key is ever loaded
+    // without rows or pages the map still needs an address and an extent of 1: packed calls load no key then, paged ones
+    // only no_page, which lies outside that extent
+    if (d->kv_tokens == 0) base = p.q;
     const uint64_t dims[4] = {d->head_dim, d->kv_heads, paged ? d->page_size : rows, rows};
     const uint64_t strides[3] = {hs, ts, 2 * (i ? d->v_page_stride : d->k_page_stride)};
     const uint32_t box[4] = {64, 1, paged ? std::min<uint32_t>(d->page_size, keys) : keys, 1};
@@ -378,6 +380,7 @@ int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* d, const void* q, c
   p.table_columns = static_cast<int>(d->table_columns);
   p.table_stride = d->table_stride;
   p.page_shift = log2_exact(d->page_size);
+  p.no_page = static_cast<int>(std::max(1u, d->kv_tokens));
   p.status = status_word();
   if (!p.status) return 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -28,6 +28,7 @@ struct AttnParams {
   int num_seqs, q_tokens, max_q, q_heads, kv_heads, group, head_dim;
   int kv_tokens;  // packed: rows of k, v; paged: pages
   int page_shift, table_columns;
+  int no_page;  // paged: a page number outside the tensor maps (they have one page at least), whose rows load as zeros
   int64_t table_stride;
   int causal;
   float scale;  // of the scores, in natural units

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     const RowsPlace begin = at;
     for (int u = 0; u < count; ++u) {
       const int stage = u % kStages;
-      int page = p.kv_tokens;  // outside the cache: zeros
+      int page = p.no_page;
       const int key = at.tile * kRowsKeys + box * box_rows;
       if (on && key < at.len_k) {
         const int id = __ldg(p.block_table + at.seq * p.table_stride + (key >> p.page_shift));

@@ -511,15 +511,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tma_load_4d(smem + L::kQ + s * L::kTile + h * 16384, &q_map, q_full + s, h * 64, 0, w.head, w.q0 + t.first[s]);
           }
         };
-        // The page of this lane's box of key tile j (outside the cache for what lies behind the last key: zeros)
+        // The page of this lane's box of key tile j (no_page for what lies behind the last key)
         const int box_rows = kPaged ? min(1 << p.page_shift, kTcKeys) : kTcKeys;
         auto page_of = [&](int j) {
           const int key = j * kTcKeys + lane * box_rows;
-          if (!kPaged || lane * box_rows >= kTcKeys || key >= t.key_end) return p.kv_tokens;
+          if (!kPaged || lane * box_rows >= kTcKeys || key >= t.key_end) return p.no_page;
           const int id = __ldg(p.block_table + w.seq * p.table_stride + (key >> p.page_shift));
           if (id >= 0 && id < p.kv_tokens) return id;
           atomicOr(p.status, kAttnBadPage);
-          return p.kv_tokens;
+          return p.no_page;
         };
         // one K or V tile; the bytes count whole boxes, what lies outside the tensor arrives as zeros
         auto load_kv = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* bar, int j, int page) {

@@ -1,0 +1,67 @@
+"""Attention over token sequences at the borders of what its entry points accept: extreme scales and values, non-finite values that
+meet, empty caches, sums near 2^31, other streams, long items."""
+import math
+
+import pytest
+import torch
+
+from aexrt_b200 import _native, ops
+from tests import _attention as oracle
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(gen, *shape, dtype, std=1.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * std).to(dtype)
+
+
+def paged_of(k, v, page=16):
+    """One sequence's keys and values in a cache of their own: (k_cache, v_cache, block table)."""
+    n, pages = k.shape[0], -(-k.shape[0] // page)
+    kc, vc = (torch.zeros(pages, page, *k.shape[1:], dtype=k.dtype, device="cuda") for _ in range(2))
+    kc.flatten(0, 1)[:n], vc.flatten(0, 1)[:n] = k, v
+    return kc, vc, torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+
+
+def every_way(q, k, v, scale, causal, news):
+    """The same attention through every kernel: yields (name, out, lse, rows) for the packed call over q and for the last `new` rows
+    of q over a cache, for each of `news`."""
+    n, cu = k.shape[0], ints([0, q.shape[0]])
+    yield ("packed", *ops.attention_packed(q, k, v, cu, ints([0, n]), causal=causal, scale=scale, return_lse=True),
+           slice(0, q.shape[0]))
+    kc, vc, table = paged_of(k, v)
+    for new in news:
+        yield (f"paged {new}", *ops.attention_paged(q[-new:], kc, vc, table, ints([0, new]), ints([n]), new, causal=causal, scale=scale,
+                                                    return_lse=True), slice(q.shape[0] - new, q.shape[0]))
+    assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,lens", [(1, [0, 0]), (1, [40, 0]), (5, [5, 300]), (90, [0, 90]), (70, [3000, 70])])
+def test_an_empty_cache_reads_as_zeros(new, lens, dtype):
+    """A cache of no pages: rows without keys give 0 and -inf, keys of table entries are zeros, and q's memory is no cache."""
+    g = generator(20)
+    hq, hk, d, page = 8, 2, 128, 16
+    q = rand(g, 2 * new, hq, d, dtype=dtype)
+    kc, vc = (torch.empty(0, page, hk, d, dtype=dtype, device="cuda") for _ in range(2))
+    columns = -(-max(lens) // page)
+    table = torch.zeros(2, columns, dtype=torch.int32, device="cuda")
+    out, lse = ops.attention_paged(q, kc, vc, table, ints([0, new, 2 * new]), ints(lens), new, return_lse=True)
+    assert ops.attention_status() == (ops.ATTENTION_BAD_PAGE if columns else 0)
+    assert bool((out == 0).all())
+    i = torch.arange(new, device="cuda")
+    seen = torch.cat([(i + 1 + n - new).clamp(0, n) for n in lens])
+    want = torch.log(seen.double())[:, None].expand(-1, hq)  # equal scores of 0
+    empty = torch.isinf(want)
+    assert torch.equal(lse[empty].double(), want[empty])
+    assert bool(((lse - want)[~empty].abs() <= seen.max() * 2.0 ** -23 + 2.0 ** -20).all())
