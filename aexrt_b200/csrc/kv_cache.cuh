@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
     p.state_out[0] = max(0, top - all);
     p.state_out[1] = max(0, all - top);
   }
-  for (int g = at; g < all; g += step) {
+  for (int64_t next = at; next < all; next += step) {  // `all` may be 2^31 - 1: a step past it needs 64 bits
+    const int g = static_cast<int>(next);
     const int s = find_request(taken, n, g);
     const int col = static_cast<int>((ctx[s] + ps - 1) >> p.page_shift) + (g - taken[s]);
     p.table[s * p.table_stride + col] = g < top ? __ldg(p.free_pages + top - 1 - g) : -1;

@@ -65,3 +65,33 @@ def test_an_empty_cache_reads_as_zeros(new, lens, dtype):
     empty = torch.isinf(want)
     assert torch.equal(lse[empty].double(), want[empty])
     assert bool(((lse - want)[~empty].abs() <= seen.max() * 2.0 ** -23 + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("capacity", [40, 200000])
+def test_tables_of_nearly_2_31_new_pages(capacity):
+    """Pages of one token and an empty stack: the last pages are written, none beyond them."""
+    columns, top = 2 ** 30, 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 12 * 2 ** 30:
+        pytest.skip("needs 12 GB")
+    base = torch.full((2 * columns + 2,), 7, dtype=torch.int32, device="cuda")
+    table = base[1:-1].view(2, columns)
+    free = ints([5, 6, 9])
+    cu, kv, slots, state = ops.page_tables(ints([0, 0]), ints([columns, columns]), table, free, ints([3, 0]), 1, max_tokens=capacity)
+    assert cu.tolist() == [0, columns, top] and state.tolist() == [0, top - 3]
+    assert table[0, :4].tolist() == [9, 6, 5, -1] and slots[:4].tolist() == [9, 6, 5, -1]
+    assert int((base == -1).sum()) == top - 3 and int((slots == -1).sum()) == capacity - 3
+    assert base[[0, -1, -2]].tolist() == [7, 7, 7]  # the sums end at 2^31 - 1: the last column is not taken
+
+
+def test_tables_of_most_requests_in_place():
+    """The largest shared memory in one cluster of blocks."""
+    n = 16384
+    g = torch.Generator().manual_seed(21)
+    ctx, new = (torch.randint(0, high, (n,), generator=g).tolist() for high in (40, 3))
+    table = [[1000 + c for c in range(6)] for _ in range(n)]
+    want = oracle.tables(ctx, new, table, list(range(20000)), 20000, 8, sum(new))
+    lens, t, state = ints(ctx), ints(table), ints([20000, 0])
+    cu, kv, slots, state_out = ops.page_tables(lens, ints(new), t, ints(list(range(20000))), state, 8, max_tokens=sum(new), kv_lens=lens,
+                                               free_state_out=state)
+    for got, exp in zip((cu, kv, t, slots, state_out), want):
+        assert got.tolist() == [list(x) if isinstance(x, (list, tuple)) else x for x in exp]
