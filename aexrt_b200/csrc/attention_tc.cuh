@@ -390,7 +390,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int first = splits && most > 1 ? with_part(0) : 0;  // the items that are split
       int part = 0;             // of the numbers that are handed out now, their first, and how many there are
       int64_t part_start = 0, part_count = all;
-      // Finds item number k of this CTA and puts it out, once every role has left item k - 2.
+      bool last = false;  // the item that ends the roles is out
+      // Finds item number k of this CTA and puts it out, once every role has left item k - 2; false: that wait gave up.
       auto publish = [&](int k) {
         int64_t number = static_cast<int64_t>(k) * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         if (splits) {
@@ -429,7 +430,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mbar_arrive(w_full + (k & 1));
         }
         __syncwarp();
-        return found;
+        last = !found;
+        return true;
       };
       // V tiles that have to be cleaned before their product.  P is 0 where a row does not see a key, but
       // 0 * inf and 0 * NaN are not: rows behind the last key become zeros (as far as the product goes, a
@@ -476,12 +478,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return true;
       };
       // two items are out at a time; an item's tiles are cleaned once the next one is out
-      bool more = publish(0) && publish(1);
-      for (int k = 0;; ++k) {
+      bool ok = publish(0) && (last || publish(1));
+      for (int k = 0; ok; ++k) {
         const TcWork w = work[k & 1];
         __syncwarp();
         if (w.head < 0 || !clean(k, w)) break;
-        more = more && publish(k + 2);
+        if (!last) ok = publish(k + 2);
       }
       if (kSplit && blockIdx.x == 0) {  // for the joining
         int base = 0;
