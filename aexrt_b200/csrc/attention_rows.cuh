@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     const bool on = is_v < 2;
     bool ok = true;
     const RowsPlace begin = at;
-    for (int u = 0; u < count; ++u) {
+    int u = 0;
+    for (; u < count; ++u) {
       const int stage = u % kStages;
       int page = p.no_page;
       const int key = at.tile * kRowsKeys + box * box_rows;
@@ -231,11 +232,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       }
       rp.runs[c] = r;
     }
-    // the loads in flight land before the block ends: the last ones of each stage
-    for (int i = 0; i < kStages && !ok; ++i) {
-      mbar_wait_bounded(full + i, 0, p.status, kAttnTimeout);
-      mbar_wait_bounded(full + i, 1, p.status, kAttnTimeout);
-    }
+    // after a wait that gave up, the loads in flight land before the block ends: the last ones of each stage
+    for (int i = max(0, u - kStages); i < u && !ok; ++i)
+      mbar_wait_bounded(full + i % kStages, (i / kStages) & 1, p.status, kAttnTimeout);
     grid_dep_launch();
     return;
   }

@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // ---------------------------------------------------------------- loads
       const uint32_t q_bytes = static_cast<uint32_t>(tokens * p.group * 128 * kHalves);
       bool ok = true;
-      int it = 0, qs[2] = {0, 0};
+      int it = 0, qs[2] = {0, 0};        // ring items and Q tiles loaded
+      uint32_t raws = 0, raw_last = 0;  // per slot: loads onto the barrier `raw`, modulo 2, and whether the last load was one
       TcWork w;
       for (int k = 0; ok; ++k) {
         ok = __all_sync(~0u, wait(w_full + (k & 1), k >> 1));
@@ -506,8 +507,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const TcTiles<kSplit> t(p, w, tokens);
         auto load_q = [&](int s) {
           if (!t.n[s] || !ok) return;
-          ok = __all_sync(~0u, wait(q_empty + s, qs[s]++ + 1));
-          if (lane == 0 && ok) {
+          ok = __all_sync(~0u, wait(q_empty + s, qs[s] + 1));
+          if (!ok) return;
+          ++qs[s];
+          if (lane == 0) {
             mbar_arrive_expect_tx(q_full + s, q_bytes);
             for (int h = 0; h < kHalves; ++h)
               tma_load_4d(smem + L::kQ + s * L::kTile + h * 16384, &q_map, q_full + s, h * 64, 0, w.head, w.q0 + t.first[s]);
@@ -553,6 +556,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           load_kv(is_v ? &v_map : &k_map, smem + L::kRing + slot * L::kTile, dirty ? raw + slot : kv_full + slot, j,
                   is_v && i + 1 < 2 * t.nmax ? page_v : page_k);
+          raw_last = dirty ? raw_last | 1u << slot : raw_last & ~(1u << slot);
+          if (dirty) raws ^= 1u << slot;
           if (kPaged && !is_v) page_next = page_of(j + 1);
           if (i == 0) load_q(1);
         }
@@ -560,12 +565,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(w_empty + (k & 1));
       }
       if (!ok) {
-        // a wait gave up: the loads in flight still have to land before the CTA may leave
-        for (uint64_t* bar : {kv_full, raw, q_full})
-          for (int i = 0; i < (bar == q_full ? 2 : NS); ++i) {
-            mbar_wait_bounded(bar + i, 0, p.status, kAttnTimeout);
-            mbar_wait_bounded(bar + i, 1, p.status, kAttnTimeout);
-          }
+        // a wait gave up: the loads in flight still have to land before the CTA may leave, which are at most the last
+        // ones of each slot (a barrier that nothing is loaded onto would cost its whole limit)
+        for (int slot = 0; slot < min(NS, it); ++slot)
+          if ((raw_last >> slot) & 1) wait(raw + slot, static_cast<int>(raws >> slot) + 1);
+          else wait(kv_full + slot, (it - 1 - slot) / NS);
+        for (int s = 0; s < 2; ++s)
+          if (qs[s]) wait(q_full + s, qs[s] - 1);
       }
     } else if (lane == 0) {
       // ---------------------------------------------------------------- MMA issue, one thread per row tile
