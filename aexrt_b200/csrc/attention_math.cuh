@@ -13,12 +13,21 @@ constexpr float kLazyLog2 = 8.f;
 // give finite probabilities.
 constexpr float kLargeLog2 = 4096.f;
 
+// Keys that one accumulator of a tensor-core product takes.  Such a sum cuts every product to 2^-25 of what is summed
+// so far before it adds it (measured: ones are lost from 2^26 on, products below 2^-10 beside 65504), so n keys can
+// lose n * 2^-25 of sum |p v|: 2^-11 of it here, half a step of fp16.  Then the sums go to fp32 ones, which round.
+constexpr int kSumKeys = 16384;
+
 // 2^x on the special-function unit (subnormal results flush to 0).
 __device__ __forceinline__ float exp2_sfu(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Sums that were taken against the maximum `from` count this much against `to`, which is not below it (equal ones,
+// infinite ones too: 1).
+__device__ __forceinline__ float moved(float from, float to, float sl2) { return from == to ? 1.f : exp2_sfu((from - to) * sl2); }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;

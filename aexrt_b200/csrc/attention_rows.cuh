@@ -247,6 +247,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   uint32_t qf[DP / 16][4];
   float o[DP / 8][4];
   float m[2], l[2];
+  // the stretches of kSumKeys keys before the one in o, against their own maxima: volatile keeps them out of the registers
+  volatile float carry[DP / 2];
+  float carry_m[2];
+  int stretch = 0;  // units in o
+  bool carried = false;
   int seen[2], common = 0, rows = 0, q0 = 0, len_q = 0;
   bool fresh = true, dead = false;
   int part_first = at.tile;  // first tile of the current (sequence, head) that this run takes
@@ -281,7 +286,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
       part_first = at.tile;
-      fresh = false;
+      fresh = carried = false;
+      stretch = 0;
     }
     // after a wait that gave up, the warp goes on without waiting (the status tells): the barriers between the
     // warps still see all of them
@@ -396,8 +402,26 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     }
 
 
+    const bool end = at.tile + 1 == at.tiles || u + 1 == count;
+    if (++stretch == kSumKeys / kWarpKeys || (end && carried)) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[e] = carried ? moved(carry_m[e], m[e], sl2) : 0.f;
+        carry_m[e] = m[e];
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 2; ++i) {
+        const float sum = carried ? fmaf(carry[i], f[(i >> 1) & 1], o[i / 4][i % 4]) : o[i / 4][i % 4];
+        if (!end) carry[i] = sum;
+        o[i / 4][i % 4] = end ? sum : 0.f;
+      }
+      carried = true;
+      stretch = 0;
+    }
+
     // ---- the end of a (sequence, head), or of the run: join the key warps, write
-    if (at.tile + 1 == at.tiles || u + 1 == count) {
+    if (end) {
       const bool whole = part_first == 0 && at.tile + 1 == at.tiles;
       const int slot = 2 * blockIdx.x + (part_first == 0 ? 1 : 0);
 #pragma unroll

@@ -51,6 +51,7 @@ constexpr int kTcThreads = 384;
 // Items of fewer key tiles stay whole: below, the joining costs more than the split saves (100 tokens over 300 cached
 // keys: 19 us whole, 22 in parts of 2 tiles).
 constexpr int kTcMinTiles = 6;
+constexpr int kTcStretch = kSumKeys / kTcKeys;  // key tiles that O sums in TMEM
 
 // Slots of the K / V ring: what 227 KB hold beside the two Q tiles and the output staging.
 template <int DP>
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               const int quarters = tc_quarters(keys, begin + j);
 #pragma unroll
               for (int c = 0; c < kTcKeys / 16; ++c)
-                if (c < quarters * 2) tc_mma_ts(o_at, p_at + c * 8, b + c * (2048 >> 4), id_o, (j | c) != 0);
+                if (c < quarters * 2) tc_mma_ts(o_at, p_at + c * 8, b + c * (2048 >> 4), id_o, (j % kTcStretch | c) != 0);
               tc_commit(o_done + s);
               tc_commit(kv_empty + i % NS);
             } else if (ok) {
@@ -667,94 +668,117 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int seen = mine ? keys_seen(token, w.len_q, w.len_k, p.causal) : 0;
       const int all_see = valid ? keys_seen(first, w.len_q, w.len_k, p.causal) : 0;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < n; ++j, ++done) {
-        ok = __all_sync(~0u, wait(s_full + s, done));
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t x[128];
+      // The stretches before the one in TMEM, against their own maximum.  In local memory (the loops that use it index
+      // it), out of the way of the registers: a row of more than kSumKeys keys needs it once a stretch.
+      float carry[DP], carry_m = -INFINITY;
+      bool carried = false;
+      for (int j = 0; j < n;) {
+        const int start = j, stop = min(n, j + kTcStretch);
+        for (; j < stop; ++j, ++done) {
+          ok = __all_sync(~0u, wait(s_full + s, done));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t x[128];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(lanes + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
-        tmem_ld_wait();
-        tc_fence_before();
-        mbar_arrive(s_free + s);
-        if ((begin + j + 1) * kTcKeys > all_see) {
-          const int lim = seen - (begin + j) * kTcKeys;
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32(lanes + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + c * 32));
+          tmem_ld_wait();
+          tc_fence_before();
+          mbar_arrive(s_free + s);
+          if ((begin + j + 1) * kTcKeys > all_see) {
+            const int lim = seen - (begin + j) * kTcKeys;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            // bit i: the row sees column 32 c + i (columns that the product left out are never seen)
-            const uint32_t sees = lim >= 32 * c + 32 ? ~0u : (lim <= 32 * c ? 0u : (1u << (lim - 32 * c)) - 1u);
+            for (int c = 0; c < 4; ++c) {
+              // bit i: the row sees column 32 c + i (columns that the product left out are never seen)
+              const uint32_t sees = lim >= 32 * c + 32 ? ~0u : (lim <= 32 * c ? 0u : (1u << (lim - 32 * c)) - 1u);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(sees & (1u << e))) x[32 * c + e] = 0xff800000u;
+              for (int e = 0; e < 32; ++e)
+                if (!(sees & (1u << e))) x[32 * c + e] = 0xff800000u;
+            }
           }
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 128; c += 8)
+          for (int c = 0; c < 128; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
-        const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
-        const bool move = (top - m) * sl2 > kLazyLog2;  // from -inf too
-        if (__any_sync(~0u, move)) {
-          const float old = m;
-          if (move) m = top;
-          const float f = move ? exp2_sfu((old - m) * sl2) : 1.f;
-          l *= f;
-          if (__any_sync(~0u, move && old != -INFINITY)) {
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
+          const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
+          const bool move = (top - m) * sl2 > kLazyLog2;  // from -inf too
+          if (__any_sync(~0u, move)) {
+            const float old = m;
+            if (move) m = top;
+            const float f = move ? exp2_sfu((old - m) * sl2) : 1.f;
+            l *= f;
+            if (__any_sync(~0u, move && old != -INFINITY)) {
+              ok = __all_sync(~0u, wait(o_done + s, done - 1));
+              if (!ok) break;
+              tc_fence_after();
+              uint32_t o[16];
+#pragma unroll 1
+              for (int c = 0; c < DP; c += 16) {
+                tmem_ld_32x16(o_at + c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st_32x16(o_at + c, o);
+              }
+              tmem_st_wait();
+            }
+          }
+          const float m0 = m == -INFINITY ? 0.f : m;
+          float base = -m0 * sl2;
+          const bool large = fabsf(base) > kLargeLog2;  // row by row: no row's result depends on its neighbours
+          if (__any_sync(~0u, large)) {
+            const float first = large ? m0 : 0.f;
+#pragma unroll
+            for (int c = 0; c < 128; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - first);
+            if (large) base = 0.f;
+          }
+          const uint64_t base2 = f2_pack(base, base), sl22 = f2_pack(sl2, sl2);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) {
+            float a, b;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sl22, base2), a, b);
+            a = exp2_sfu(a);
+            b = exp2_sfu(b);
+            sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
+            x[c >> 1] = pack16<T>(a, b);
+          }
+          if (j > start) {  // the last P has been consumed
             ok = __all_sync(~0u, wait(o_done + s, done - 1));
             if (!ok) break;
             tc_fence_after();
-            uint32_t o[16];
-#pragma unroll 1
-            for (int c = 0; c < DP; c += 16) {
-              tmem_ld_32x16(o_at + c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st_32x16(o_at + c, o);
-            }
-            tmem_st_wait();
           }
-        }
-        const float m0 = m == -INFINITY ? 0.f : m;
-        float base = -m0 * sl2;
-        const bool large = fabsf(base) > kLargeLog2;  // row by row: no row's result depends on its neighbours
-        if (__any_sync(~0u, large)) {
-          const float first = large ? m0 : 0.f;
-#pragma unroll
-          for (int c = 0; c < 128; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - first);
-          if (large) base = 0.f;
-        }
-        const uint64_t base2 = f2_pack(base, base), sl22 = f2_pack(sl2, sl2);
-        uint64_t sum[2] = {0, 0};
-#pragma unroll
-        for (int c = 0; c < 128; c += 2) {
+          tmem_st_32x32(p_at, x);
+          tmem_st_32x32(p_at + 32, x + 32);
           float a, b;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sl22, base2), a, b);
-          a = exp2_sfu(a);
-          b = exp2_sfu(b);
-          sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
-          x[c >> 1] = pack16<T>(a, b);
+          f2_unpack(f2_add(sum[0], sum[1]), a, b);
+          l += a + b;
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(p_full + s);
         }
-        if (j > 0) {  // the last P has been consumed
-          ok = __all_sync(~0u, wait(o_done + s, done - 1));
-          if (!ok) break;
-          tc_fence_after();
-        }
-        tmem_st_32x32(p_at, x);
-        tmem_st_32x32(p_at + 32, x + 32);
-        float a, b;
-        f2_unpack(f2_add(sum[0], sum[1]), a, b);
-        l += a + b;
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(p_full + s);
+        if (!ok || j == n) break;
+        ok = __all_sync(~0u, wait(o_done + s, done - 1));  // the next tile's product starts O anew
+        if (!ok) break;
+        tc_fence_after();
+        const float f = moved(carry_m, m, sl2);
+        uint32_t o[16];
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 16) {
+          tmem_ld_32x16(o_at + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) carry[c + e] = carried ? fmaf(carry[c + e], f, __uint_as_float(o[e])) : __uint_as_float(o[e]);
+      }
+      carry_m = m;
+      carried = true;
       }
       if (ok && n) ok = __all_sync(~0u, wait(o_done + s, done - 1));
       if (ok && valid) {
         tc_fence_after();
         const bool part = kSplit && w.part >= 0;
         const float inv = part ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        const float carry_f = moved(carry_m, m, sl2);
         const int64_t tok = w.q0 + token;
         const int qh = w.head * p.group + row_head;
         const uint64_t dst = reinterpret_cast<uint64_t>(static_cast<T*>(p.out) + tok * p.o_ts + qh * p.o_hs);
@@ -773,6 +797,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             } else {
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if (carried) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(fmaf(carry[c + e], carry_f, __uint_as_float(o[e])));
             }
             if (seen == 0) {
 #pragma unroll
@@ -823,6 +851,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (n) {
               tmem_ld_32x32(o_at + c, o);
               tmem_ld_wait();
+            }
+            if (carried) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(fmaf(carry[c + e], carry_f, __uint_as_float(o[e])));
             }
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = n && seen ? o[e] : 0u;

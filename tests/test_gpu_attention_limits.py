@@ -95,3 +95,37 @@ def test_tables_of_most_requests_in_place():
                                                free_state_out=state)
     for got, exp in zip((cu, kv, t, slots, state_out), want):
         assert got.tolist() == [list(x) if isinstance(x, (list, tuple)) else x for x in exp]
+
+
+def test_sums_over_many_keys_keep_their_small_terms():
+    """One value of 65504 and many of about 2^-10 with equal probabilities.  A tensor-core sum cuts each product to 2^-25 of what is
+    summed so far, so that the small ones vanish beside the large one unless the keys are summed in stretches.  The bound: 2^14
+    products a stretch, each cut by 2^-25 of the sum at most, 2^10 sums of 16 cut by 2^-23, some hundred stretches added in fp32, and
+    the output's rounding.  Probabilities are 1, so they and their sum are exact."""
+    d, small, page = 64, 0.99 * 2.0 ** -10, 1024
+
+    def check(out, lse, n, what):
+        v = torch.full((1,), small, dtype=F16, device="cuda").double()
+        want = (65504 + (n - 1) * v) / n
+        over = (out.double() - want).abs() / (want * (2.0 ** -11 + 2.0 ** -13 + 2.0 ** -16 + 2.0 ** -11))
+        assert bool((over <= 1).all()), f"{what}: {float(over.max()):.3g} of the bound"
+        assert bool(((lse - math.log(n)).abs() <= 2.0 ** -19).all()), what
+
+    n = 2 ** 18
+    for rows in (1, 200):
+        q = torch.zeros(rows, 1, d, dtype=F16, device="cuda")
+        k = torch.zeros(n, 1, d, dtype=F16, device="cuda")
+        v = torch.full((n, 1, d), small, dtype=F16, device="cuda")
+        v[5] = 65504
+        check(*ops.attention_packed(q, k, v, ints([0, rows]), ints([0, n]), causal=False, return_lse=True), n, ("packed", rows))
+    # a cache of two pages, the second one repeated; as many sequences as there are blocks, so that no item is split
+    kc = torch.zeros(2, page, 1, d, dtype=F16, device="cuda")
+    vc = torch.full((2, page, 1, d), small, dtype=F16, device="cuda")
+    vc[0, 5] = 65504
+    for seqs, n, rows in ((300, 2 ** 20, 1), (300, 2 ** 20, 40), (300, 2 ** 17, 80)):
+        table = torch.ones(seqs, n // page, dtype=torch.int32, device="cuda")
+        table[:, 0] = 0
+        q = torch.zeros(seqs * rows, 1, d, dtype=F16, device="cuda")
+        cu = ints([i * rows for i in range(seqs + 1)])
+        check(*ops.attention_paged(q, kc, vc, table, cu, ints([n] * seqs), rows, causal=False, return_lse=True), n, ("paged", rows))
+    assert ops.attention_status() == 0
