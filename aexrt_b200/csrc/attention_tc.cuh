@@ -301,6 +301,28 @@ __device__ __forceinline__ void mbar_arrive_count(uint64_t* bar, uint32_t count)
                : "memory");
 }
 
+// A wait that lasts while others work: it gives up when neither the barrier nor the loading warp (*beat, its ring items)
+// has moved for the limit's clocks.  An item may take longer than any limit (40 million keys pass half a second), and
+// some roles wait for most of one.  The ring is finite, so a loading warp that goes on means products that go on.
+__device__ __forceinline__ bool mbar_wait_beat(uint64_t* bar, uint32_t parity, uint32_t* status, const volatile int* beat) {
+  if (mbar_test_wait(bar, parity)) return true;
+  int seen = *beat;
+  long long t0 = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      if (*beat == seen) {
+        atomicOr(status, kAttnTimeout);
+        return false;
+      }
+      seen = *beat;
+      t0 = clock64();
+    }
+  }
+}
+
 // Quarters of 32 keys that a row tile needs of key tile j when its last row sees `keys` keys: products and
 // softmax of the last tile stop there.
 __device__ __forceinline__ int tc_quarters(int keys, int j) { return min(4, (keys - j * kTcKeys + 31) >> 5); }
@@ -323,6 +345,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
            *drain = s_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* fixed = reinterpret_cast<int*>(tmem_slot + 1);  // [2]
+  volatile int* beat = fixed + 2;
   TcWork* work = reinterpret_cast<TcWork*>(fixed + 3);  // [2]
   int* fix = reinterpret_cast<int*>(smem + L::kFix);    // [2][kFixInts]
   static_assert((14 + 3 * tc_slots<DP>() + 4) * 8 + 16 + 2 * sizeof(TcWork) <= 640, "barriers and items fit");
@@ -347,6 +370,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(kv_empty + i, 2);
       mbar_init(raw + i, 1);
     }
+    *beat = 0;
     fence_mbar_init();
   }
   for (int i = threadIdx.x; i < 2 * kFixInts; i += kTcThreads) fix[i] = INT_MAX;
@@ -360,7 +384,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int tokens = kTcRows / p.group;  // query tokens of a row tile
-  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait_bounded(bar, phase & 1, p.status, kAttnTimeout); };
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait_beat(bar, phase & 1, p.status, beat); };
   // Item number k of this CTA, once it is known; head -1 ends the roles (so does a wait that gave up).
   auto item = [&](int k, TcWork& w) {
     const bool ok = wait(w_full + (k & 1), k >> 1);
@@ -559,6 +583,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   is_v && i + 1 < 2 * t.nmax ? page_v : page_k);
           raw_last = dirty ? raw_last | 1u << slot : raw_last & ~(1u << slot);
           if (dirty) raws ^= 1u << slot;
+          if (lane == 0) *beat = it;
           if (kPaged && !is_v) page_next = page_of(j + 1);
           if (i == 0) load_q(1);
         }

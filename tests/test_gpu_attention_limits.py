@@ -129,3 +129,21 @@ def test_sums_over_many_keys_keep_their_small_terms():
         cu = ints([i * rows for i in range(seqs + 1)])
         check(*ops.attention_paged(q, kc, vc, table, cu, ints([n] * seqs), rows, causal=False, return_lse=True), n, ("paged", rows))
     assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("extra", [0, 37])
+def test_an_item_of_more_than_a_hundred_million_keys(extra):
+    """One row over so many keys that its one block works for longer than any wait's limit.  Equal scores: probabilities of 1, whose sums
+    are exact below 2^27 (steps of 8 for sums of 16), so the outputs are shares of n, rounded once."""
+    n, tail, d = 2 ** 27 - 4096 + extra, 2 ** 22, 8
+    q = torch.ones(1, 1, d, dtype=F16, device="cuda")
+    k = torch.zeros(n, 1, d, dtype=F16, device="cuda")
+    v = torch.zeros(n, 1, d, dtype=F16, device="cuda")
+    v[:, :, 0] = 1
+    v[-tail:, :, 1] = 1
+    v[:tail, :, 2] = 1
+    out, lse = ops.attention_packed(q, k, v, ints([0, 1]), ints([0, n]), causal=False, return_lse=True)
+    assert ops.attention_status() == 0
+    want = torch.tensor([1.0, tail / n, tail / n] + [0.0] * 5, dtype=torch.float64, device="cuda")
+    assert bool(((out[0, 0].double() - want).abs() <= want * (2.0 ** -11 + 2.0 ** -22)).all())
+    assert abs(float(lse[0, 0]) - math.log(n)) <= 2.0 ** -19  # one step of fp32 at 18.7
