@@ -15,6 +15,7 @@ PyTorch fallback for any of them.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import struct
 from dataclasses import dataclass
@@ -442,16 +443,35 @@ def _call(fn, what: str, torch, tensors, stream, args):
     return fn(*args, handle)
 
 
-def _outputs(what: str, torch, q, q_shape, out, lse, return_lse):
+def _allocating(torch, stream, device):
+    """The context in which a call on `stream` allocates: that stream's own, since memory from the current one's pool may
+    still be used by work that is queued there.  (Tensors that are not on a GPU are refused by the call.)"""
+    if stream is None or device.type != "cuda":
+        return contextlib.nullcontext()
+    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream)
+                             else torch.cuda.ExternalStream(_stream(stream), device=device))
+
+
+def _made(torch, stream, shape, dtype, device):
+    """A tensor that a call on `stream` writes and returns: not reused before both that stream and the current one have
+    passed its last use."""
+    with _allocating(torch, stream, device):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if stream is not None and t.is_cuda:
+        t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
+def _outputs(what: str, torch, q, q_shape, out, lse, return_lse, stream):
     """The outputs given or made: (out, its strides, lse)."""
     if out is None:
-        out = torch.empty(q_shape, dtype=q.dtype, device=q.device)
+        out = _made(torch, stream, q_shape, q.dtype, q.device)
     shape, strides = _heads(out, what, "out", 3)
     if shape != q_shape or out.dtype is not q.dtype:
         raise ValueError(f"{what}: out must have q's shape and type")
     if lse is None:
         if return_lse:
-            lse = torch.empty(q_shape[:2], dtype=torch.float32, device=q.device)
+            lse = _made(torch, stream, q_shape[:2], torch.float32, q.device)
     elif lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape != q_shape[:2] or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor [tokens, heads]")
     return out, strides, lse
@@ -469,7 +489,7 @@ def attention_packed(q, k, v, cu_q, cu_k, causal: bool = True, scale: Optional[f
     tokens, heads, dim = q_shape
     k_shape, ks = _heads(k, what, "k", 3)
     v_shape, vs = _heads(v, what, "v", 3)
-    out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse)
+    out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse, stream)
     if k_shape != v_shape or k_shape[2] != dim or not q.dtype is k.dtype is v.dtype:
         raise ValueError(f"{what}: k and v must have one shape, and q's type and head size")
     num_seqs = cu_q.shape[0] - 1
@@ -512,7 +532,7 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
     tokens, heads, dim = q_shape
     k_shape, ks = _heads(k_cache, what, "k_cache", 4)
     v_shape, vs = _heads(v_cache, what, "v_cache", 4)
-    out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse)
+    out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse, stream)
     if k_shape != v_shape or k_shape[3] != dim or not q.dtype is k_cache.dtype is v_cache.dtype:
         raise ValueError(f"{what}: the caches must have one shape, and q's type and head size")
     num_seqs = kv_lens.shape[0]
@@ -520,9 +540,8 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
         raise ValueError(f"{what}: max_q must not be negative")
     table, columns, table_stride = _table(block_table, what, num_seqs, torch.int32)
     if workspace is None:
-        workspace = attention_paged_workspace(q, k_cache, num_seqs, max_q)
-        if stream is not None and workspace.numel():  # not reused before that stream has passed the call
-            workspace.record_stream(torch.cuda.ExternalStream(_stream(stream), device=q.device))
+        with _allocating(torch, stream, q.device):
+            workspace = attention_paged_workspace(q, k_cache, num_seqs, max_q)
     elif not workspace.is_contiguous():
         raise ValueError(f"{what}: workspace must be contiguous")
     desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1 if causal else 0,
@@ -556,7 +575,7 @@ def page_tables(ctx_lens, new_lens, block_table, free_pages, free_state, page_si
     n = ctx_lens.shape[0]
 
     def ints(size):
-        return torch.empty((size,), dtype=torch.int32, device=ctx_lens.device)
+        return _made(torch, stream, (size,), torch.int32, ctx_lens.device)
 
     if slot_map is None:
         if max_tokens is None:

@@ -147,3 +147,63 @@ def test_an_item_of_more_than_a_hundred_million_keys(extra):
     want = torch.tensor([1.0, tail / n, tail / n] + [0.0] * 5, dtype=torch.float64, device="cuda")
     assert bool(((out[0, 0].double() - want).abs() <= want * (2.0 ** -11 + 2.0 ** -22)).all())
     assert abs(float(lse[0, 0]) - math.log(n)) <= 2.0 ** -19  # one step of fp32 at 18.7
+
+
+def busy(*shapes):
+    """Work queued on the current stream that will write NaN (or -1) into memory which is free for the next tensors of these shapes."""
+    tensors = [torch.zeros(s, dtype=t, device="cuda") for s, t in shapes]
+    torch.cuda._sleep(200_000_000)  # a tenth of a second
+    for t in tensors:
+        t.fill_(math.nan if t.dtype.is_floating_point else -1)
+
+
+@pytest.mark.parametrize("handle", [False, True])
+@pytest.mark.parametrize("new", [1, 90])
+def test_tensors_made_for_another_stream_are_not_in_use_here(new, handle):
+    """Calls on a side stream that make their outputs and workspaces, while the current stream still has work queued on memory
+    that it has freed."""
+    g = generator(22)
+    q, n = rand(g, new, 8, 128, dtype=BF16, std=2.0), 6000
+    k, v = (rand(g, n, 2, 128, dtype=BF16) for _ in range(2))
+    kc, vc, table = paged_of(k, v)
+    cu, lens, cu_k = ints([0, new]), ints([n]), ints([0, n])
+    want = oracle.attend_block(q, k, v, 128 ** -0.5, True)
+    size = ops.attention_paged_workspace(q, kc, 1, new).numel()
+    side = torch.cuda.Stream()
+    stream = side.cuda_stream if handle else side
+    torch.cuda.synchronize()
+    shapes = ((q.shape, BF16), (q.shape[:2], torch.float32), ((size,), torch.uint8))
+    busy(*shapes)
+    got = [ops.attention_paged(q, kc, vc, table, cu, lens, new, return_lse=True, stream=stream)]
+    busy(*shapes)
+    got.append(ops.attention_packed(q, k, v, cu, cu_k, return_lse=True, stream=stream))
+    torch.cuda.synchronize()
+    for out, lse in got:
+        oracle.check(out, lse, *want)
+    made, allocate = [], ops.attention_paged_workspace
+
+    def spy(*args):
+        made.append((torch.cuda.current_stream().cuda_stream, allocate(*args)))
+        return made[-1][1]
+
+    ops.attention_paged_workspace = spy  # the workspace is taken where it is used
+    try:
+        ops.attention_paged(q, kc, vc, table, cu, lens, new, stream=stream)
+    finally:
+        ops.attention_paged_workspace = allocate
+    assert [s for s, _ in made] == [side.cuda_stream]
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+
+
+def test_tables_made_for_another_stream_are_not_in_use_here():
+    n = 300
+    ctx, new, table = ints([20] * n), ints([1] * n), torch.full((n, 4), 9, dtype=torch.int32, device="cuda")
+    free, state = ints(list(range(50))), ints([50, 0])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    i32 = torch.int32
+    busy(((n + 1,), i32), ((n,), i32), ((n,), i32), ((2,), i32))
+    cu, kv, slots, state = ops.page_tables(ctx, new, table, free, state, 16, max_tokens=n, stream=side)
+    torch.cuda.synchronize()
+    assert cu.tolist() == list(range(n + 1)) and kv.tolist() == [21] * n
+    assert slots.tolist() == [9 * 16 + 4] * n and state.tolist() == [50, 0]
