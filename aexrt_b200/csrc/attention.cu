@@ -44,7 +44,10 @@ bool cuda_ok(cudaError_t e, const char* what) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-static __device__ uint32_t g_attention_status;
+static __device__ uint32_t g_attention_status[2];  // the status word, and what the last read took out of it
+
+// Reads and clears in one step: bits set meanwhile are neither lost nor seen twice.
+__global__ void take_status_kernel(uint32_t* word) { word[1] = atomicExch(word, 0u); }
 
 // This device's status word, its address resolved once per device.
 uint32_t* status_word() {
@@ -391,8 +394,13 @@ int aexrt_b200_attention_status(uint32_t* status) {
   if (!status) return fail("attention_status: null pointer");
   uint32_t* word = status_word();
   if (!word) return 0;
-  if (!cuda_ok(cudaMemcpy(status, word, sizeof(uint32_t), cudaMemcpyDeviceToHost), "read status")) return 0;
-  return cuda_ok(cudaMemset(word, 0, sizeof(uint32_t)), "clear status") ? 1 : 0;
+  // the default stream does not wait for streams made without that tie, as torch's are
+  if (!cuda_ok(cudaDeviceSynchronize(), "synchronize for the attention status")) return 0;
+  static std::mutex mu;  // one reader at a time: the kernel and the copy of what it took
+  std::lock_guard<std::mutex> lock(mu);
+  take_status_kernel<<<1, 1>>>(word);
+  if (!cuda_ok(cudaGetLastError(), "attention status launch")) return 0;
+  return cuda_ok(cudaMemcpy(status, word + 1, sizeof(uint32_t), cudaMemcpyDeviceToHost), "read attention status") ? 1 : 0;
 }
 
 int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uint32_t num_seqs, uint32_t page_size,

@@ -556,7 +556,7 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
 
 
 def attention_status() -> int:
-    """Reads and clears the attention kernels' status word of the current device (ATTENTION_* bits)."""
+    """Reads and clears the attention kernels' status word of the current device (ATTENTION_* bits), after all work on it, on any stream."""
     v = ctypes.c_uint32(0)
     check(_native.load().aexrt_b200_attention_status(ctypes.byref(v)), "attention_status")
     return v.value

@@ -510,8 +510,8 @@ int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* desc, const void* q
 /* Workspace bytes of the call on the current device; ~0 for a description that the call refuses. */
 uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* desc);
 
-/* Status of this device's attention kernels since the last read: reads and clears it
- * (synchronises).  BAD_PAGE: a block table entry outside the cache was met.  TIMEOUT: a wait inside
+/* Status of the current device's attention kernels since the last read: waits for all work on the
+ * device, on every stream, then reads and clears it in one step (so not while a stream is captured).  BAD_PAGE: a block table entry outside the cache was met.  TIMEOUT: a wait inside
  * a kernel gave up, and outputs of that call are incomplete. */
 #define AEXRT_B200_ATTENTION_BAD_PAGE 1u
 #define AEXRT_B200_ATTENTION_TIMEOUT 2u

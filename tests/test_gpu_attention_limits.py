@@ -207,3 +207,37 @@ def test_tables_made_for_another_stream_are_not_in_use_here():
     torch.cuda.synchronize()
     assert cu.tolist() == list(range(n + 1)) and kv.tolist() == [21] * n
     assert slots.tolist() == [9 * 16 + 4] * n and state.tolist() == [50, 0]
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_status_covers_calls_on_side_streams(new):
+    """A bad table entry met by a call that is still to run when the status is asked for."""
+    g = generator(23)
+    q = rand(g, new, 2, 64, dtype=F16)
+    kc, vc, table = paged_of(*(rand(g, 200, 2, 64, dtype=F16) for _ in range(2)))
+    table[0, 3] = -1
+    cu, lens = ints([0, new]), ints([200])
+    ws = ops.attention_paged_workspace(q, kc, 1, new)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert ops.attention_status() == 0
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        ops.attention_paged(q, kc, vc, table, cu, lens, new, workspace=ws)
+    assert ops.attention_status() == ops.ATTENTION_BAD_PAGE
+    assert ops.attention_status() == 0
+
+
+def test_status_is_read_by_one_of_many_readers():
+    from concurrent.futures import ThreadPoolExecutor
+
+    g = generator(24)
+    q = rand(g, 1, 2, 64, dtype=F16)
+    kc, vc, table = paged_of(*(rand(g, 40, 2, 64, dtype=F16) for _ in range(2)))
+    table[0, 1] = kc.shape[0]
+    assert ops.attention_status() == 0
+    with ThreadPoolExecutor(8) as pool:
+        for _ in range(20):
+            ops.attention_paged(q, kc, vc, table, ints([0, 1]), ints([40]), 1)
+            got = list(pool.map(lambda _: ops.attention_status(), range(8)))
+            assert sorted(got) == [0] * 7 + [ops.ATTENTION_BAD_PAGE]
