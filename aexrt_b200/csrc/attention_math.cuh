@@ -87,10 +87,11 @@ __device__ __forceinline__ uint4 take_non_finite(uint4 x, int key, int d0, int* 
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// What a row that sees keys 0 .. seen - 1 gets in a column from values that were taken out.
+// A row's output o in a column, with the values added that were taken out and that it sees (keys 0 .. seen - 1).  Sums:
+// what the other keys gave may be infinite or NaN itself.
 __device__ __forceinline__ float put_back(float o, const int* fix, int col, int seen) {
   const bool up = fix[col] < seen, down = fix[128 + col] < seen;
-  return up ? (down ? __int_as_float(0x7fffffff) : INFINITY) : (down ? -INFINITY : o);
+  return o + (up ? (down ? __int_as_float(0x7fffffff) : INFINITY) : (down ? -INFINITY : 0.f));
 }
 constexpr int kFixInts = 2 * 128;
 

@@ -241,3 +241,31 @@ def test_status_is_read_by_one_of_many_readers():
             ops.attention_paged(q, kc, vc, table, ints([0, 1]), ints([40]), 1)
             got = list(pool.map(lambda _: ops.attention_status(), range(8)))
             assert sorted(got) == [0] * 7 + [ops.ATTENTION_BAD_PAGE]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("keys", [300, 20000])
+@pytest.mark.parametrize("first,last", [(-math.inf, math.inf), (math.inf, -math.inf), (math.nan, math.inf), (math.inf, math.inf)])
+def test_infinities_that_meet(first, last, keys, dtype):
+    """An infinity of V that every row of a tile sees, and one near the end that only the last rows see: the rows that see both get
+    what their sum is."""
+    g = generator(4)
+    q = rand(g, 80, 4, 64, dtype=dtype)
+    k, v = (rand(g, keys, 2, 64, dtype=dtype) for _ in range(2))
+    v[0, 0, 3] = v[1, 1, 40] = first
+    v[-1, 0, 3] = v[-3, 1, 40] = last
+    want = oracle.attend(q, k, v, 0.125, True)
+    for name, out, lse, rows in every_way(q, k, v, 0.125, True, (1, 2, 15, 80)):
+        oracle.check(out, lse, *[w[rows] for w in want], name)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_an_infinite_value_in_a_row_of_nan_scores(dtype):
+    g = generator(5)
+    q = rand(g, 80, 2, 64, dtype=dtype)
+    k, v = (rand(g, 300, 2, 64, dtype=dtype) for _ in range(2))
+    k[5, 0], v[-1, 0, 7] = math.nan, math.inf
+    want = oracle.attend(q, k, v, 0.125, True)
+    assert bool(torch.isnan(want[0][:, 0]).all())
+    for name, out, lse, rows in every_way(q, k, v, 0.125, True, (1, 2, 80)):
+        oracle.check(out, None, *[w[rows] for w in want], name)
