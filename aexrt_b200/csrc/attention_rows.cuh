@@ -443,8 +443,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
           float all = -INFINITY;  // the row's maximum over the key warps
 #pragma unroll
           for (int w = 0; w < kKeyWarps; ++w) all = fmaxf(all, stat[((w * MT + wr) * 16 + g + 8 * e) * 2]);
-          // equal maxima, infinite ones too: 1
-          const float f = m[e] == all ? 1.f : (m[e] == -INFINITY ? 0.f : exp2_sfu((m[e] - all) * sl2));
+          const float f = moved(m[e], all, sl2);
           float* row = join + (warp * 16 + g + 8 * e) * DP;
 #pragma unroll
           for (int n = 0; n < DP / 8; ++n)
@@ -463,7 +462,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         for (int w = 0; w < kKeyWarps; ++w) {
           const int at_row = (w * MT + (r >> 4)) * 16 + (r & 15);
           const float2 st = *reinterpret_cast<const float2*>(stat + at_row * 2);
-          norm += st.x == all ? st.y : (st.x == -INFINITY ? 0.f : st.y * exp2_sfu((st.x - all) * sl2));
+          norm += st.y * moved(st.x, all, sl2);  // NaN from a warp whose scores are all NaN (maximum -inf) too
           const float4* src = reinterpret_cast<const float4*>(join + at_row * DP + (c ^ ((r & 7) << 3)));
           const float4 a = src[0], b = src[1];
           y[0] += a.x, y[1] += a.y, y[2] += a.z, y[3] += a.w, y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;

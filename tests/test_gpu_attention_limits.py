@@ -269,3 +269,18 @@ def test_an_infinite_value_in_a_row_of_nan_scores(dtype):
     assert bool(torch.isnan(want[0][:, 0]).all())
     for name, out, lse, rows in every_way(q, k, v, 0.125, True, (1, 2, 80)):
         oracle.check(out, None, *[w[rows] for w in want], name)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("keys", [17, 33, 49, 65, 81, 700])
+def test_a_nan_score_reaches_lse(keys, dtype):
+    """The last key alone is NaN, wherever the computing warps' shares of a unit end."""
+    g = generator(3)
+    q = rand(g, 1, 4, 64, dtype=dtype)
+    k, v = (rand(g, keys, 2, 64, dtype=dtype) for _ in range(2))
+    k[-1, 1] = math.nan
+    want = oracle.attend(q, k, v, 0.125, True)
+    assert bool(torch.isnan(want[1][:, 2:]).all())
+    for name, out, lse, rows in every_way(q, k, v, 0.125, True, (1,)):
+        assert torch.equal(torch.isnan(out), torch.isnan(want[0])), name
+        assert torch.equal(torch.isnan(lse), torch.isnan(want[1])), name
