@@ -301,24 +301,21 @@ __device__ __forceinline__ void mbar_arrive_count(uint64_t* bar, uint32_t count)
                : "memory");
 }
 
-// A wait that lasts while others work: it gives up when neither the barrier nor the loading warp (*beat, its ring items)
-// has moved for the limit's clocks.  An item may take longer than any limit (40 million keys pass half a second), and
-// some roles wait for most of one.  The ring is finite, so a loading warp that goes on means products that go on.
+// A wait that may last an item: it gives up when neither the barrier nor the loading warp (*beat, its ring items) has
+// moved for the limit's clocks.  An item may take longer than any limit (40 million keys pass half a second).  The ring is
+// finite, so a loading warp that goes on means products that go on.  Only where it is needed: the finding warp's waits, and
+// the softmax warps' for an item or its first scores, whose tile may have no part in the item before.  All other waits are
+// over within a few key tiles (in every wait of the kernel it made ragged prompts 9 % slower).
 __device__ __forceinline__ bool mbar_wait_beat(uint64_t* bar, uint32_t parity, uint32_t* status, const volatile int* beat) {
-  if (mbar_test_wait(bar, parity)) return true;
-  int seen = *beat;
-  long long t0 = clock64();
   while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i)
+    const int seen = *beat;
+    const long long t0 = clock64();
+    do {
       if (mbar_try_wait(bar, parity)) return true;
-    if (clock64() - t0 > kWaitLimitCycles) {
-      if (*beat == seen) {
-        atomicOr(status, kAttnTimeout);
-        return false;
-      }
-      seen = *beat;
-      t0 = clock64();
+    } while (clock64() - t0 <= kWaitLimitCycles);
+    if (*beat == seen) {
+      atomicOr(status, kAttnTimeout);
+      return false;
     }
   }
 }
@@ -384,10 +381,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int tokens = kTcRows / p.group;  // query tokens of a row tile
-  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait_beat(bar, phase & 1, p.status, beat); };
+  auto wait = [&](uint64_t* bar, int phase) { return mbar_wait_bounded(bar, phase & 1, p.status, kAttnTimeout); };
+  auto wait_long = [&](uint64_t* bar, int phase) { return mbar_wait_beat(bar, phase & 1, p.status, beat); };
   // Item number k of this CTA, once it is known; head -1 ends the roles (so does a wait that gave up).
-  auto item = [&](int k, TcWork& w) {
-    const bool ok = wait(w_full + (k & 1), k >> 1);
+  auto item = [&](int k, TcWork& w, bool may_last) {
+    const bool ok = may_last ? wait_long(w_full + (k & 1), k >> 1) : wait(w_full + (k & 1), k >> 1);
     w = work[k & 1];
     return ok && w.head >= 0;
   };
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             w.part = static_cast<int>(number + (part ? first + part_start - all : 0));
           }
         }
-        if (!__all_sync(~0u, wait(w_empty + (k & 1), (k >> 1) + 1))) return false;
+        if (!__all_sync(~0u, wait_long(w_empty + (k & 1), (k >> 1) + 1))) return false;
         const bool used = fixed[k & 1] != 0;
         __syncwarp();
         if (used) {  // by item k - 2
@@ -471,7 +469,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int begin = kSplit ? w.begin : 0, sub = lane >> 3, piece = lane & 7;
         for (int j = max(t.unclean - begin, 0); j < t.nmax; ++j) {
           const int slot = (it + (j + 1 < t.nmax ? 2 * j + 2 : 2 * t.nmax - 1)) % NS, key = (begin + j) * kTcKeys;
-          if (!__all_sync(~0u, wait(raw + slot, (raws >> slot) & 1))) return false;
+          if (!__all_sync(~0u, wait_long(raw + slot, (raws >> slot) & 1))) return false;
           raws ^= 1u << slot;
           const int last = min(t.key_end - key, kTcKeys), from = max(0, min(t.common - key, last));
           for (int h = 0; h < kHalves; ++h) {
@@ -613,7 +611,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int it = 0, qs = 0, ps = 0;
       auto full = [&](int i) { return wait(kv_full + i % NS, i / NS); };
       TcWork w;
-      for (int k = 0; ok && item(k, w); ++k) {
+      for (int k = 0; ok && item(k, w, false); ++k) {
         const TcTiles<kSplit> t(p, w, tokens);
         const int n = s ? t.n[1] : t.n[0], keys = s ? t.keys[1] : t.keys[0], begin = kSplit ? w.begin : 0;
         // every ring item in order, K0 K1 V0 K2 V1 ..., also those that only the other tile uses
@@ -685,7 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool ok = true;
     int done = 0;  // key tiles of this row tile so far, over all items
     TcWork w;
-    for (int k = 0; ok && __all_sync(~0u, item(k, w)); ++k) {
+    for (int k = 0; ok && __all_sync(~0u, item(k, w, true)); ++k) {
       const TcTiles<kSplit> t(p, w, tokens);
       const int first = s ? t.first[1] : t.first[0], valid = s ? t.valid[1] : t.valid[0], n = s ? t.n[1] : t.n[0];
       const int token = first + row_token, begin = kSplit ? w.begin : 0;
@@ -697,7 +695,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // it), out of the way of the registers: a row of more than kSumKeys keys needs it once a stretch.
       float carry[DP], carry_m = -INFINITY;
       bool carried = false;
-      for (int j = 0; j < n;) {
+      if (n) ok = __all_sync(~0u, wait_long(s_full + s, done));
+      for (int j = 0; ok && j < n;) {
         const int start = j, stop = min(n, j + kTcStretch);
         for (; j < stop; ++j, ++done) {
           ok = __all_sync(~0u, wait(s_full + s, done));
