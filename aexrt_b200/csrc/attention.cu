@@ -126,7 +126,7 @@ bool desc_ok(const AexrtB200AttentionDesc* d, bool paged) {
   if (d->q_heads == 0 || d->kv_heads == 0 || d->q_heads > 65535u || d->q_heads % d->kv_heads)
     return fail("%s: q_heads must be a multiple of kv_heads, from 1 to 65535", what) != 0;
   if (d->q_heads / d->kv_heads > 128) return fail("%s: at most 128 query heads per kv head", what) != 0;
-  if (!(d->scale >= 0.f) || !std::isfinite(d->scale)) return fail("%s: scale must be finite and >= 0", what) != 0;
+  if (!(d->scale >= 0.f) || d->scale > 1e38f) return fail("%s: scale must be from 0 to 1e38", what) != 0;
   if (d->q_tokens > (1u << 30) || d->kv_tokens > (1u << 30)) return fail("%s: at most 2^30 rows or pages", what) != 0;
   // rows x heads index the launch grids
   if (static_cast<uint64_t>(d->q_tokens) * d->q_heads > (1ull << 32))
@@ -180,7 +180,7 @@ AttnParams make_params(const AexrtB200AttentionDesc* d, const void* q, const voi
   p.head_dim = static_cast<int>(d->head_dim);
   p.kv_tokens = static_cast<int>(d->kv_tokens);
   p.causal = d->causal ? 1 : 0;
-  p.scale = d->scale;
+  p.scale = std::max(d->scale, kMinScale);
   return p;
 }
 

@@ -14,6 +14,10 @@ namespace aexrt {
 // Bits of the attention status word (AEXRT_B200_ATTENTION_*).
 enum : uint32_t { kAttnBadPage = 1u << 0, kAttnTimeout = 1u << 1 };
 
+// What a scale of 0 is replaced by, fp32's smallest number: 0 would make NaN of a masked score's -inf.  The largest score
+// becomes 2^-21, as much as rounding its exponential may take.
+constexpr float kMinScale = 1.401298464e-45f;
+
 struct AttnParams {
   const void *q, *k, *v;  // k, v: packed rows or the paged caches
   void* out;
@@ -31,7 +35,7 @@ struct AttnParams {
   int no_page;  // paged: a page number outside the tensor maps (they have one page at least), whose rows load as zeros
   int64_t table_stride;
   int causal;
-  float scale;  // of the scores, in natural units
+  float scale;  // of the scores, in natural units: kMinScale to 1e38, so that scale * log2 e is neither 0 nor infinite
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }

@@ -16,7 +16,7 @@ struct JoinHead {
 template <typename T, typename RowOf>
 __device__ __forceinline__ void join_row(const AttnParams& p, const float* sums, const float* stats, int parts, RowOf row_of, int d,
                                          int token, int qh) {
-  const float scale = fmaxf(p.scale, 1e-30f), sl2 = scale * 1.4426950408889634f;
+  const float sl2 = p.scale * 1.4426950408889634f;
   float y[8] = {}, all = -INFINITY, norm = 0.f;
   for (int k0 = 0; k0 < parts; k0 += 4) {
     float2 st[4];
@@ -52,7 +52,7 @@ __device__ __forceinline__ void join_row(const AttnParams& p, const float* sums,
   *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + token * p.o_ts + qh * p.o_hs + d) =
       make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
   if (d == 0 && p.lse)
-    p.lse[static_cast<int64_t>(token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
+    p.lse[static_cast<int64_t>(token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm));
 }
 
 }  // namespace aexrt

@@ -239,8 +239,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     return;
   }
 
-  const float scale = fmaxf(p.scale, 1e-30f);  // 0 would make NaN of a masked score's -inf
-  const float sl2 = scale * 1.4426950408889634f;
+  const float sl2 = p.scale * 1.4426950408889634f;
   const int steps = (p.head_dim + 15) / 16;
   const int g = lane >> 2, quad = lane & 3;
 
@@ -479,7 +478,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
           *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + c) =
               make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
           if (c == 0 && p.lse)
-            p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, scale, logf(norm));
+            p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm));
         } else {
           const int64_t part = static_cast<int64_t>(slot) * rp.rows + r;
           float4* dst = reinterpret_cast<float4*>(rp.parts + part * p.head_dim + c);

@@ -678,8 +678,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int row_token = row / p.group, row_head = row % p.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 TMEM lanes
     const uint32_t p_at = lanes + 128 + s * 64, o_at = lanes + 256 + s * 128;
-    const float scale = fmaxf(p.scale, 1e-30f);  // 0 would make NaN of a masked score's -inf
-    const float sl2 = scale * 1.4426950408889634f;
+    const float sl2 = p.scale * 1.4426950408889634f;
     bool ok = true;
     int done = 0;  // key tiles of this row tile so far, over all items
     TcWork w;
@@ -908,7 +907,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           if (mine) *reinterpret_cast<float2*>(split.stats + (static_cast<int64_t>(w.part) * 256 + s * 128 + row) * 2) = make_float2(m, l);
         } else if (mine && p.lse) {
-          p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, scale, logf(l));
+          p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, p.scale, logf(l));
         }
         tc_fence_before();  // these reads of O before the next item's first product into it
       }

@@ -480,7 +480,7 @@ typedef struct AexrtB200AttentionDesc {
     uint32_t max_q;       /* paged only: the most query tokens of one sequence; later ones are left out */
     uint32_t q_heads, kv_heads, head_dim;
     uint32_t causal;
-    float scale;          /* finite, >= 0 */
+    float scale;          /* 0 to 1e38 */
     uint32_t kv_tokens;   /* packed: rows of k and v.  paged: pages of the cache */
     uint32_t page_size;   /* paged: tokens per page, a power of two from 8 to 1024 */
     uint32_t table_columns, table_stride; /* paged: columns of block_table (times page_size at most 2^30), elements

@@ -284,3 +284,38 @@ def test_a_nan_score_reaches_lse(keys, dtype):
     for name, out, lse, rows in every_way(q, k, v, 0.125, True, (1,)):
         assert torch.equal(torch.isnan(out), torch.isnan(want[0])), name
         assert torch.equal(torch.isnan(lse), torch.isnan(want[1])), name
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -130, 2.0 ** -120, 2.0 ** -90])
+def test_small_scales_of_large_scores(scale):
+    """Scores near the end of fp32 under scales down to 0: the scaled scores are what counts."""
+    g = generator(1)
+    n, d = 300, 64
+    q, k = ((torch.rand(n, 2, d, generator=g, device="cuda") + 0.5).mul(1e18).to(BF16) for _ in range(2))
+    k = torch.where(torch.rand(n, 2, 1, generator=g, device="cuda") < 0.5, k, -k)  # scores of both signs, about 6e37
+    v = rand(g, n, 2, d, dtype=BF16)
+    want = oracle.attend_block(q, k, v, scale, True)
+    for name, out, lse, rows in every_way(q, k, v, scale, True, (1, 5, 80)):
+        oracle.check(out, lse, *[w[rows] for w in want], name)
+
+
+def test_large_scales_of_small_scores():
+    """The largest scale, over scores of 1e-35."""
+    g = generator(2)
+    n, d, scale = 300, 64, float(torch.tensor(1e38))  # as fp32 holds it
+    q, k = ((torch.rand(n, 2, d, generator=g, device="cuda") + 1).mul(1e-18).to(BF16) for _ in range(2))
+    k = torch.where(torch.rand(n, 2, d, generator=g, device="cuda") < 0.5, k, -k)  # no product is subnormal
+    v = rand(g, n, 2, d, dtype=BF16)
+    want = oracle.attend_block(q, k, v, scale, True)
+    for name, out, lse, rows in every_way(q, k, v, scale, True, (1, 5, 80)):
+        oracle.check(out, lse, *[w[rows] for w in want], name)
+
+
+@pytest.mark.parametrize("scale", [1.01e38, 3e38])
+def test_scales_whose_exponents_pass_fp32_are_refused(scale):
+    q = torch.zeros(1, 1, 8, dtype=BF16, device="cuda")
+    with pytest.raises(_native.AexrtError, match="scale must be from 0 to 1e38"):
+        ops.attention_packed(q, q, q, ints([0, 1]), ints([0, 1]), scale=scale)
+    kc, vc, table = paged_of(q, q)
+    with pytest.raises(_native.AexrtError, match="scale must be from 0 to 1e38"):
+        ops.attention_paged(q, kc, vc, table, ints([0, 1]), ints([1]), 1, scale=scale)
