@@ -50,7 +50,7 @@ __device__ __forceinline__ void join_row(const AttnParams& p, const float* sums,
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] *= inv;
   *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + token * p.o_ts + qh * p.o_hs + d) =
-      make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+      make_uint4(pack_out<T>(y[0], y[1]), pack_out<T>(y[2], y[3]), pack_out<T>(y[4], y[5]), pack_out<T>(y[6], y[7]));
   if (d == 0 && p.lse)
     p.lse[static_cast<int64_t>(token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm));
 }

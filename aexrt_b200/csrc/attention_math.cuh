@@ -50,6 +50,16 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   return r;
 }
 
+// An output as its type holds it.  It is an average of finite values, or infinite because one of them is: the
+// probabilities' rounding may take an fp16 average of up to 65504 past 65520, which would round to infinity.
+template <typename T>
+__device__ __forceinline__ float in_range(float o) {
+  if constexpr (__is_same(T, __half)) return fabsf(o) < 66000.f ? fminf(fmaxf(o, -65504.f), 65504.f) : o;
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) { return pack16<T>(in_range<T>(lo), in_range<T>(hi)); }
+
 // A word of two 16-bit values with an infinity or NaN among them: the exponent field of all ones
 // carries into the sign bit.
 template <typename T>

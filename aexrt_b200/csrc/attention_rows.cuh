@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         }
         if (whole) {
           *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + c) =
-              make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+              make_uint4(pack_out<T>(y[0], y[1]), pack_out<T>(y[2], y[3]), pack_out<T>(y[4], y[5]), pack_out<T>(y[6], y[7]));
           if (c == 0 && p.lse)
             p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm));
         } else {

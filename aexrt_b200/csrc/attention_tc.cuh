@@ -839,7 +839,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 o[31] = __float_as_uint(y);
               }
             }
-            const float f = patch ? 1.f : inv;
+            float f = patch ? 1.f : inv;
+            if constexpr (__is_same(T, __half)) {  // 32 at a time: 90.0 us for 16 maps of 1600 positions, value by value 91.2
+              float big = 0.f;
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) big = max3(big, fabsf(__uint_as_float(o[e])), fabsf(__uint_as_float(o[e + 1])));
+              if (big * f > 65504.f) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(in_range<T>(__uint_as_float(o[e]) * f));
+                f = 1.f;
+              }
+            }
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               uint32_t y[4];

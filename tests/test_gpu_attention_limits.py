@@ -319,3 +319,34 @@ def test_scales_whose_exponents_pass_fp32_are_refused(scale):
     kc, vc, table = paged_of(q, q)
     with pytest.raises(_native.AexrtError, match="scale must be from 0 to 1e38"):
         ops.attention_paged(q, kc, vc, table, ints([0, 1]), ints([1]), 1, scale=scale)
+
+
+def test_fp16_averages_of_its_largest_value_stay_finite():
+    """Every value 65504: an average cannot pass it, whatever the probabilities' rounding adds up to.  Scores a over the second half of
+    the keys, 0 over the first, so that the later probabilities are e^a as fp16 rounds it."""
+    n, heads, d = 512, 16, 64
+    rows = 40
+    a = torch.linspace(0.1, 5.0, rows * heads, device="cuda").reshape(rows, heads)
+    q = torch.zeros(rows, heads, d, dtype=F16, device="cuda")
+    q[..., 0] = a.to(F16)
+    k = torch.zeros(n, 1, d, dtype=F16, device="cuda")
+    k[n // 2:, :, 0] = 1
+    v = torch.full((n, 1, d), 65504.0, dtype=F16, device="cuda")
+    v[:, :, d // 2:] = -65504.0
+    want = oracle.attend_block(q, k, v, 1.0, False)
+    for name, out, lse, at in every_way(q, k, v, 1.0, False, (1, 2, 4, 40)):
+        assert bool(torch.isfinite(out).all()), name
+        oracle.check(out, lse, *[w[at] for w in want], name)
+    # many (sequence, head) pairs, so that a block keeps several units of each
+    seqs = 400
+    kc, vc, table = paged_of(k, v)
+    a = torch.linspace(0.1, 5.0, seqs * heads, device="cuda").reshape(seqs, heads)
+    q = torch.zeros(seqs, heads, d, dtype=F16, device="cuda")
+    q[..., 0] = a.to(F16)
+    out = ops.attention_paged(q, kc, vc, table.expand(seqs, -1).contiguous(), ints(list(range(seqs + 1))), ints([n] * seqs), 1, scale=1.0)
+    assert bool(torch.isfinite(out).all())
+    # infinite values stay what they are
+    v[3, 0, 0], v[4, 0, d - 1] = math.inf, -math.inf
+    for name, out, lse, at in every_way(q[:40], k, v, 1.0, False, (1, 40)):
+        assert bool((out[..., 0] == math.inf).all()) and bool((out[..., d - 1] == -math.inf).all()), name
+        assert bool(torch.isfinite(out[..., 1:d - 1]).all()), name
