@@ -4,9 +4,17 @@
 
 namespace aexrt {
 
-// A row's maximum may run ahead of the reference that its probabilities are taken against by 2^8: they
-// stay below 2^8, far inside fp16, and most tiles need no rescaling of the accumulators.
+// A row's maximum may run ahead of the reference that its probabilities are taken against by 2^8, so that most tiles need
+// no rescaling of the accumulators.
 constexpr float kLazyLog2 = 8.f;
+
+// P is held in the tensors' 16-bit type, as the tensor cores take it; the normaliser is summed from the unrounded values.
+// In fp16 it is taken 2^7 times larger (up to 2^15 with the above): its steps end at 2^-24, and many keys of 2^-25 of the
+// largest probability, which round to 0 there, may count together.  bf16 has fp32's range.
+template <typename T>
+constexpr float kProbLog2 = __is_same(T, __half) ? 7.f : 0.f;
+template <typename T>
+constexpr float kProbUnit = __is_same(T, __half) ? 1.f / 128 : 1.f;
 
 // s * c - m * c as one multiply-add carries the rounding of m * c, half a step of its own magnitude: 2^-12 here.
 // Beyond, s - m is taken first (exact for the scores that count), so that scores as large as fp32 holds still

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     for (int n = 0; n < kWarpKeys / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[n][e] = exp2_sfu((s[n][e] - m0[e >> 1]) * sl2);  // the difference first: finite for any finite scores
+        s[n][e] = exp2_sfu(fmaf(s[n][e] - m0[e >> 1], sl2, kProbLog2<T>));  // the difference first: finite for any finite scores
         l[e >> 1] += s[n][e];
       }
     // ---- O += P V
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
           *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + c) =
               make_uint4(pack_out<T>(y[0], y[1]), pack_out<T>(y[2], y[3]), pack_out<T>(y[4], y[5]), pack_out<T>(y[6], y[7]));
           if (c == 0 && p.lse)
-            p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm));
+            p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm * kProbUnit<T>));
         } else {
           const int64_t part = static_cast<int64_t>(slot) * rp.rows + r;
           float4* dst = reinterpret_cast<float4*>(rp.parts + part * p.head_dim + c);

@@ -11,7 +11,7 @@
 // (with P in S's place each tile's P V, the next S and their latency, 1400 clocks, followed the 1850 of its
 // softmax: 1040 TFLOP/s).  A thread owns a row, so the running maximum m and sum l need no exchange
 // between threads.  O in TMEM is in units of a reference maximum that moves only when a row's true
-// maximum has passed it by 2^8: P stays below 2^8 (far inside fp16) and the rescaling of O, a
+// maximum has passed it by 2^8: P stays inside fp16 and the rescaling of O, a
 // round trip through registers, is skipped for almost every tile.
 //
 // A 128 x 128 tile costs 1024 clocks of exp on the special-function units (16 a clock), as many as its
@@ -747,13 +747,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
           const float m0 = m == -INFINITY ? 0.f : m;
-          float base = -m0 * sl2;
-          const bool large = fabsf(base) > kLargeLog2;  // row by row: no row's result depends on its neighbours
+          const float top2 = m0 * sl2;
+          float base = kProbLog2<T> - top2;
+          const bool large = fabsf(top2) > kLargeLog2;  // row by row: no row's result depends on its neighbours
           if (__any_sync(~0u, large)) {
             const float first = large ? m0 : 0.f;
 #pragma unroll
             for (int c = 0; c < 128; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - first);
-            if (large) base = 0.f;
+            if (large) base = kProbLog2<T>;
           }
           const uint64_t base2 = f2_pack(base, base), sl22 = f2_pack(sl2, sl2);
           uint64_t sum[2] = {0, 0};
@@ -917,7 +918,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           if (mine) *reinterpret_cast<float2*>(split.stats + (static_cast<int64_t>(w.part) * 256 + s * 128 + row) * 2) = make_float2(m, l);
         } else if (mine && p.lse) {
-          p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, p.scale, logf(l));
+          p.lse[tok * p.q_heads + qh] = l == 0.f ? -INFINITY : fmaf(m, p.scale, logf(l * kProbUnit<T>));
         }
         tc_fence_before();  // these reads of O before the next item's first product into it
       }

@@ -350,3 +350,38 @@ def test_fp16_averages_of_its_largest_value_stay_finite():
     for name, out, lse, at in every_way(q[:40], k, v, 1.0, False, (1, 40)):
         assert bool((out[..., 0] == math.inf).all()) and bool((out[..., d - 1] == -math.inf).all()), name
         assert bool(torch.isfinite(out[..., 1:d - 1]).all()), name
+
+
+def test_fp16_keeps_the_mass_of_small_probabilities():
+    """One key far above all others, which together count: each of their probabilities is 2^-25.6 of the largest.  The bound is the
+    oracle's with its last term's step taken relative to probabilities of up to 2^7: n 2^-32 V."""
+    def check(out, k, v, q, what):
+        s = (q.double() @ k.double().T)
+        p = torch.exp(s - s.max())
+        p /= p.sum()
+        want, size, n = p @ v.double(), p @ v.double().abs(), k.shape[0]
+        u = oracle.half_step(F16)
+        tol = size * (u + 2 * 2.0 ** -17 + n * 2.0 ** -22) + u * want.abs() + n * 2.0 ** -32 * v.double().abs().max() + 2.0 ** -25
+        # scores: one product each, exact in fp32, so no term for them
+        over = (out.double() - want).abs() / tol
+        assert bool((over <= 1).all()), f"{what}: {float(over.max()):.3g} of the bound"
+
+    d = 64
+    for n, size in ((32768, 100.0), (2048, 60000.0)):
+        k = torch.zeros(n, 1, d, dtype=F16, device="cuda")
+        k[0, 0, 0] = 17.75
+        v = torch.full((n, 1, d), size, dtype=F16, device="cuda")
+        v[0] = 0
+        for rows in (1, 100):
+            q = torch.zeros(rows, 1, d, dtype=F16, device="cuda")
+            q[..., 0] = 1
+            for name, out, lse, at in every_way(q, k, v, 1.0, False, (rows,)):
+                for r in range(out.shape[0]):
+                    check(out[r, 0], k[:, 0], v[:, 0], q[at][r, 0], (name, n))
+        seqs = 300  # one block has many units of a sequence
+        kc, vc, table = paged_of(k, v)
+        q = torch.zeros(seqs, 1, d, dtype=F16, device="cuda")
+        q[..., 0] = 1
+        out = ops.attention_paged(q, kc, vc, table.expand(seqs, -1).contiguous(), ints(list(range(seqs + 1))), ints([n] * seqs), 1, scale=1.0)
+        for r in range(0, seqs, 7):
+            check(out[r, 0], k[:, 0], v[:, 0], q[r, 0], ("rows", n))
