@@ -403,6 +403,21 @@ def _dtype16(t, what: str, torch) -> int:
     raise ValueError(f"{what}: float16 or bfloat16 tensors, not {dtype}")
 
 
+def _pack(what: str, *fields) -> bytes:
+    """An AexrtB200AttentionDesc of these fields (those behind struct_size)."""
+    try:
+        return _DESC.pack(_DESC.size, *fields)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"{what}: a size or the scale is out of range ({e})") from None
+
+
+def _entries(t, what: str, name: str) -> int:
+    """The entries of a vector."""
+    if t.dim() != 1:
+        raise ValueError(f"{what}: {name} must have one dimension")
+    return t.shape[0]
+
+
 def _heads(t, what: str, name: str, dims: int):
     """Shape and strides of a [..., heads, head_dim] tensor with contiguous heads (the library ignores the stride of a
     dimension of size 1, which torch leaves arbitrary)."""
@@ -492,11 +507,11 @@ def attention_packed(q, k, v, cu_q, cu_k, causal: bool = True, scale: Optional[f
     out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse, stream)
     if k_shape != v_shape or k_shape[2] != dim or not q.dtype is k.dtype is v.dtype:
         raise ValueError(f"{what}: k and v must have one shape, and q's type and head size")
-    num_seqs = cu_q.shape[0] - 1
+    num_seqs = _entries(cu_q, what, "cu_q") - 1
     if num_seqs < 0:
         raise ValueError(f"{what}: cu_q must have at least one entry")
-    desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, 0, heads, k_shape[1], dim, 1 if causal else 0,
-                      dim ** -0.5 if scale is None else scale, k_shape[0], 0, 0, 0, qs[0], qs[1], os_[0], os_[1],
+    desc = _pack(what, _dtype16(q, what, torch), num_seqs, tokens, 0, heads, k_shape[1], dim, 1 if causal else 0,
+                      max(dim, 1) ** -0.5 if scale is None else scale, k_shape[0], 0, 0, 0, qs[0], qs[1], os_[0], os_[1],
                       ks[0], ks[1], 0, vs[0], vs[1], 0)
     check(_call(_native.load().aexrt_b200_attention_packed, what, torch, (q, k, v, cu_q, cu_k, out, lse), stream,
                 (desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), _index(cu_q, what, "cu_q", num_seqs + 1, torch.int32),
@@ -512,7 +527,7 @@ def attention_paged_workspace(q, k_cache, num_seqs: int, max_q: int):
     k_shape, ks = _heads(k_cache, what, "k_cache", 4)
     if max_q < 0:
         raise ValueError(f"{what}: max_q must not be negative")
-    desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1, 1.0, k_shape[0],
+    desc = _pack(what, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1, 1.0, k_shape[0],
                       k_shape[1], 0, 0, qs[0], qs[1], heads * dim, dim, ks[1], ks[2], ks[0], ks[1], ks[2], ks[0])
     n = _call(lambda desc, stream: _native.load().aexrt_b200_attention_paged_workspace(desc), what, torch, (q, k_cache), 0, (desc,))
     check(n != 2 ** 64 - 1, what)
@@ -535,7 +550,7 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
     out, os_, lse = _outputs(what, torch, q, q_shape, out, lse, return_lse, stream)
     if k_shape != v_shape or k_shape[3] != dim or not q.dtype is k_cache.dtype is v_cache.dtype:
         raise ValueError(f"{what}: the caches must have one shape, and q's type and head size")
-    num_seqs = kv_lens.shape[0]
+    num_seqs = _entries(kv_lens, what, "kv_lens")
     if max_q < 0:
         raise ValueError(f"{what}: max_q must not be negative")
     table, columns, table_stride = _table(block_table, what, num_seqs, torch.int32)
@@ -544,8 +559,8 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_q, kv_lens, max_q: int,
             workspace = attention_paged_workspace(q, k_cache, num_seqs, max_q)
     elif not workspace.is_contiguous():
         raise ValueError(f"{what}: workspace must be contiguous")
-    desc = _DESC.pack(_DESC.size, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1 if causal else 0,
-                      dim ** -0.5 if scale is None else scale, k_shape[0], k_shape[1], columns, table_stride,
+    desc = _pack(what, _dtype16(q, what, torch), num_seqs, tokens, max_q, heads, k_shape[2], dim, 1 if causal else 0,
+                      max(dim, 1) ** -0.5 if scale is None else scale, k_shape[0], k_shape[1], columns, table_stride,
                       qs[0], qs[1], os_[0], os_[1], ks[1], ks[2], ks[0], vs[1], vs[2], vs[0])
     check(_call(_native.load().aexrt_b200_attention_paged, what, torch,
                 (q, k_cache, v_cache, block_table, cu_q, kv_lens, out, lse, workspace), stream,
@@ -572,7 +587,7 @@ def page_tables(ctx_lens, new_lens, block_table, free_pages, free_state, page_si
     token's slot, -1 where it has no page and behind the last token.  ``kv_lens`` may be ``ctx_lens`` and
     ``free_state_out`` may be ``free_state``: updated in place, as a captured step wants them."""
     what, torch = "page_tables", _torch()
-    n = ctx_lens.shape[0]
+    n = _entries(ctx_lens, what, "ctx_lens")
 
     def ints(size):
         return _made(torch, stream, (size,), torch.int32, ctx_lens.device)
@@ -585,7 +600,9 @@ def page_tables(ctx_lens, new_lens, block_table, free_pages, free_state, page_si
     kv_lens = ints(n) if kv_lens is None else kv_lens
     free_state_out = ints(2) if free_state_out is None else free_state_out
     table, columns, table_stride = _table(block_table, what, n, torch.int32)
-    free, slots = free_pages.shape[0], slot_map.shape[0]
+    free, slots = _entries(free_pages, what, "free_pages"), _entries(slot_map, what, "slot_map")
+    if (n | page_size | columns | table_stride | free | slots) >> 32:  # a C uint32_t would cut it; negative ones too
+        raise ValueError(f"{what}: a size is out of range")
     check(_call(_native.load().aexrt_b200_page_tables, what, torch,
                 (ctx_lens, new_lens, block_table, free_pages, free_state, cu_q, kv_lens, slot_map, free_state_out), stream,
                 (_index(ctx_lens, what, "ctx_lens", n, torch.int32), _index(new_lens, what, "new_lens", n, torch.int32), n, page_size, table, columns,
@@ -609,6 +626,8 @@ def kv_append(k, v, slot_map, k_cache, v_cache, stream=None):
         raise ValueError(f"{what}: k and v, and the caches, must agree in heads and head size")
     if not k.dtype is v.dtype is k_cache.dtype is v_cache.dtype:
         raise ValueError(f"{what}: one type for k, v and the caches")
+    if (k_shape[0] | k_shape[1] | k_shape[2] | kc_shape[0] | kc_shape[1]) >> 32:  # a C uint32_t would cut it
+        raise ValueError(f"{what}: a size is out of range")
     check(_call(_native.load().aexrt_b200_kv_append, what, torch, (k, v, slot_map, k_cache, v_cache), stream,
                 (k.data_ptr(), v.data_ptr(), k_shape[0], k_shape[1], k_shape[2], ks[0], ks[1], vs[0], vs[1],
                  _index(slot_map, what, "slot_map", k_shape[0], torch.int32), k_cache.data_ptr(), v_cache.data_ptr(), kc_shape[0],
