@@ -467,7 +467,8 @@ int aexrt_b200_act_quantize_f16_noalloc(const void* x, uint32_t n, uint32_t c, u
  *   - head_dim: a multiple of 8 from 8 to 128; q_heads / kv_heads: at most 128.  Pointers 16-byte
  *     aligned, strides (elements) multiples of 8 (that of a dimension of size 1 is ignored), each
  *     head's head_dim elements contiguous.
- *     Every offset is computed in 64 bits.
+ *     Every offset is computed in 64 bits.  A stride of 0 (broadcast heads or tokens) is allowed but for out.
+ *   - out may be q itself, with its strides; otherwise out and lse overlap nothing that the call reads or writes.
  *   - Launches are asynchronous on `stream` and allocate nothing. */
 #define AEXRT_B200_DTYPE_F16 0u
 #define AEXRT_B200_DTYPE_BF16 1u
@@ -541,7 +542,7 @@ int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uin
 
 /* Writes rows k[t], v[t] ([kv_heads][head_dim] of 16-bit elements) to slot slot_map[t] of the
  * caches; slots below 0 or at and above num_pages * page_size (below 2^31) are skipped.  Two tokens
- * with the same slot leave each 16-byte piece from one of them.  Strides as in AexrtB200AttentionDesc. */
+ * with the same slot leave each 16-byte piece from one of them.  The caches overlap neither k, v nor each other.  Strides as in AexrtB200AttentionDesc. */
 int aexrt_b200_kv_append(const void* k, const void* v, uint32_t tokens, uint32_t kv_heads, uint32_t head_dim,
                          uint64_t k_token_stride, uint64_t k_head_stride, uint64_t v_token_stride,
                          uint64_t v_head_stride, const int32_t* slot_map, void* k_cache, void* v_cache,

@@ -385,3 +385,173 @@ def test_fp16_keeps_the_mass_of_small_probabilities():
         out = ops.attention_paged(q, kc, vc, table.expand(seqs, -1).contiguous(), ints(list(range(seqs + 1))), ints([n] * seqs), 1, scale=1.0)
         for r in range(0, seqs, 7):
             check(out[r, 0], k[:, 0], v[:, 0], q[r, 0], ("rows", n))
+
+
+def unit_weights(call, keys_of, lens, dim, unit=64):
+    """Equal scores and values that are 1 in one column per unit of keys: every unit's weight is read from the outputs, dim units a
+    call.  call(v_of) -> [(out row [heads, dim], lse row, seen keys, sequence)], v_of(s) the values of a sequence."""
+    units = -(-max(lens) // unit)
+    for w in range(0, units, dim):
+        def values(s):
+            n = lens[s]
+            v = torch.zeros(n, keys_of, dim, device="cuda")
+            at = torch.arange(n, device="cuda")
+            col = at // unit - w
+            on = (col >= 0) & (col < dim)
+            v[at[on], :, col[on]] = 1
+            return v
+
+        for out, lse, seen, s in call(values):
+            edges = torch.arange(w, w + dim, device="cuda") * unit
+            count = (seen - edges).clamp(0, unit).double()
+            want = count / max(seen, 1)
+            # counts are exact sums of ones; the normaliser, its reciprocal and the product round in fp32, the output once
+            tol = want * (oracle.half_step(out.dtype) + 2.0 ** -21) + 2.0 ** -25
+            assert bool(((out.double() - want).abs() <= tol).all()), (s, seen, w)
+            if seen:
+                assert bool(((lse - math.log(seen)).abs() <= 2.0 ** -19).all()), (s, seen)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens,new,hq,hk", [
+    ([33000, 11, 9000, 64, 65, 63, 1], 1, 8, 2), ([33000, 11, 9000], 3, 4, 1), ([20000, 129], 9, 16, 4), ([33000, 700, 9000], 70, 4, 2),
+    ([9000, 9001, 8999], 200, 4, 4), ([64 * i + i % 3 for i in range(1, 60)], 1, 2, 2), ([3000] * 40, 5, 6, 3)])
+def test_every_unit_of_keys_counts_once(lens, new, hq, hk, dtype):
+    """The borders between blocks' shares of the keys, in both paged kernels: no unit is lost and none is taken twice."""
+    d, page = 128, 16
+    new_of = [min(new, n) for n in lens]
+    kc, vc = (torch.zeros(sum(-(-n // page) for n in lens), page, hk, d, dtype=dtype, device="cuda") for _ in range(2))
+    table = torch.full((len(lens), -(-max(lens) // page)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(lens):
+        m = -(-n // page)
+        table[i, :m] = torch.arange(at, at + m, dtype=torch.int32, device="cuda").flip(0)
+        at += m
+    q = torch.zeros(sum(new_of), hq, d, dtype=dtype, device="cuda")
+    cu = oracle.sums(new_of)
+
+    def call(values):
+        for i, n in enumerate(lens):
+            ids = table[i, :-(-n // page)].long()
+            rows = torch.zeros(len(ids) * page, hk, d, device="cuda")
+            rows[:n] = values(i)
+            vc[ids] = rows.view(len(ids), page, hk, d).to(dtype)
+        for causal in (True, False):
+            out, lse = ops.attention_paged(q, kc, vc, table, ints(cu), ints(lens), max(new_of), causal=causal, return_lse=True)
+            for i, n in enumerate(lens):
+                for r in {0, new_of[i] - 1, new_of[i] // 2}:
+                    yield out[cu[i] + r], lse[cu[i] + r], r + 1 + n - new_of[i] if causal else n, i
+
+    unit_weights(call, hk, lens, d)
+    assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("lens", [[9000, 300], [128 * i + i for i in range(1, 20)]])
+def test_every_unit_of_a_prompt_counts_once(lens):
+    hq, hk, d = 4, 2, 64
+    cu = oracle.sums(lens)
+    q, k = (torch.zeros(cu[-1], h, d, dtype=BF16, device="cuda") for h in (hq, hk))
+
+    def call(values):
+        v = torch.cat([values(i) for i in range(len(lens))]).to(BF16)
+        for causal in (True, False):
+            out, lse = ops.attention_packed(q, k, v, ints(cu), ints(cu), causal=causal, return_lse=True)
+            for i, n in enumerate(lens):
+                for r in {0, 1, 127, n // 2, n - 2, n - 1}:
+                    yield out[cu[i] + r], lse[cu[i] + r], r + 1 if causal else n, i
+
+    unit_weights(call, hk, lens, d)
+
+
+def test_heads_and_tokens_of_stride_0():
+    """Broadcast key/value heads, a broadcast key and broadcast queries: as copies of them."""
+    g = generator(25)
+    q = rand(g, 70, 4, 64, dtype=F16)
+    k, v = (rand(g, 70, 1, 64, dtype=F16) for _ in range(2))
+    one = rand(g, 1, 4, 64, dtype=F16)
+    cu = ints([0, 70])
+    for args in ((q, k.expand(70, 4, 64), v.expand(70, 4, 64)), (q, one.expand(70, 4, 64), one.expand(70, 4, 64)),
+                 (one.expand(70, 4, 64), q, q), (q[:, :1].expand(70, 4, 64), q, q)):
+        want = ops.attention_packed(*(t.contiguous() for t in args), cu, cu, return_lse=True)
+        got = ops.attention_packed(*args, cu, cu, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    kc, vc, table = paged_of(k, v)
+    for new in (1, 70):
+        args = (q[-new:], kc.expand(-1, 16, 4, 64), vc.expand(-1, 16, 4, 64))
+        rest = (table, ints([0, new]), ints([70]), new)
+        assert torch.equal(ops.attention_paged(*args, *rest), ops.attention_paged(*(t.contiguous() for t in args), *rest))
+
+
+@pytest.mark.parametrize("n", [128, 129, 200])
+def test_many_sequences_of_many_rows_over_a_cache(n):
+    """More sequences than the tensor-core kernel orders by length, some of them empty or without new tokens."""
+    import random
+
+    rng, g = random.Random(n), generator(26)
+    new = [rng.choice([0, 1, 40, 65, 130]) for _ in range(n)]
+    lens = [x + rng.choice([0, 1, 15, 300, 1100]) if rng.random() < 0.9 else 0 for x in new]
+    hq, hk, d, page = 4, 2, 64, 32
+    need = [-(-x // page) for x in lens]
+    kc, vc = (rand(g, sum(need) + 1, page, hk, d, dtype=BF16) for _ in range(2))
+    kc[-1], vc[-1] = math.nan, math.nan
+    table = torch.full((n, max(need)), sum(need), dtype=torch.int32, device="cuda")
+    at, parts, rows = 0, [], 0
+    q = rand(g, sum(new), hq, d, dtype=BF16, std=2.0)
+    for i, m in enumerate(need):
+        ids = torch.arange(at, at + m, device="cuda")
+        table[i, :m] = ids.int()
+        at += m
+        parts.append(oracle.attend_block(q[rows:rows + new[i]], kc[ids].flatten(0, 1)[:lens[i]], vc[ids].flatten(0, 1)[:lens[i]],
+                                         0.125, True))
+        rows += new[i]
+    out = torch.full_like(q, 1000.0)
+    out, lse = ops.attention_paged(q, kc, vc, table, ints(oracle.sums(new)), ints(lens), max(new), out=out, return_lse=True)
+    assert ops.attention_status() == 0
+    oracle.check(out, lse, *[torch.cat(x) for x in zip(*parts)])
+
+
+def test_prompts_captured_and_replayed_with_other_lengths():
+    g = generator(27)
+    t, hq, hk, d, n = 900, 8, 2, 128, 6
+    q, out = (torch.zeros(t, hq, d, dtype=BF16, device="cuda") for _ in range(2))
+    k, v = (torch.zeros(t, hk, d, dtype=BF16, device="cuda") for _ in range(2))
+    lse, cu = torch.zeros(t, hq, device="cuda"), ints([0] * (n + 1))
+    ops.attention_packed(q, k, v, cu, cu, out=out, lse=lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_packed(q, k, v, cu, cu, out=out, lse=lse)
+    for lens in ([900, 0, 0, 0, 0, 0], [1, 1, 1, 1, 1, 1], [130, 256, 0, 77, 300, 1], [0] * 6, [0, 0, 0, 0, 0, 641]):
+        for x in (q, k, v):
+            x.copy_(rand(g, *x.shape, dtype=BF16))
+        cu.copy_(ints(oracle.sums(lens)))
+        out.fill_(5.0)
+        lse.fill_(7.0)
+        graph.replay()
+        s = sum(lens)
+        parts = [oracle.attend_block(a, b, c, d ** -0.5, True) for a, b, c in zip(*(torch.split(x[:s], lens) for x in (q, k, v)))]
+        oracle.check(out[:s], lse[:s], *[torch.cat(x) for x in zip(*parts)])
+        assert bool((out[s:] == 5).all()) and bool((lse[s:] == 7).all())
+    assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("new", [1, 7, 90, 400])
+def test_outputs_in_place_of_the_queries(new):
+    """out may be q."""
+    g = generator(28)
+    lens = [5000, new, 40 + new]
+    q, kv = rand(g, 3 * new, 8, 128, dtype=BF16), [(rand(g, n, 2, 128, dtype=BF16), rand(g, n, 2, 128, dtype=BF16)) for n in lens]
+    cu = ints([0, new, 2 * new, 3 * new])
+    k, v = (torch.cat(x) for x in zip(*kv))
+    want = ops.attention_packed(q, k, v, cu, ints(oracle.sums(lens)))
+    here = q.clone()
+    assert ops.attention_packed(here, k, v, cu, ints(oracle.sums(lens)), out=here) is here and torch.equal(here, want)
+    caches = [paged_of(a, b) for a, b in kv]
+    kc, vc = (torch.cat([c[i] for c in caches]) for i in (0, 1))
+    table, at = torch.full((3, max(c[2].shape[1] for c in caches)), -1, dtype=torch.int32, device="cuda"), 0
+    for i, c in enumerate(caches):
+        table[i, :c[2].shape[1]] = c[2][0] + at
+        at += c[2].shape[1]
+    want = ops.attention_paged(q, kc, vc, table, cu, ints(lens), new)
+    here = q.clone()
+    ops.attention_paged(here, kc, vc, table, cu, ints(lens), new, out=here)
+    assert torch.equal(here, want)
