@@ -33,7 +33,8 @@ struct RowsSmem {
   static constexpr int kHalf = kRowsKeys * DP * 2, kStage = 2 * kHalf;  // K, V
   static_assert(kStage == 4 * 16 * DP * 4, "a stage holds the four warps' accumulators");
   static constexpr int kStat = rows_stages<DP>() * kStage;              // m, l of each warp's rows
-  static constexpr int kFix = kStat + 4 * 16 * 2 * 4;
+  static constexpr int kPrev = kStat + 4 * 16 * 2 * 4;                  // m, l of each row's stretches before, in turn
+  static constexpr int kFix = kPrev + 2 * 64 * 2 * 4;
   static constexpr int kBars = kFix + kFixInts * 4 + 16;
   static constexpr int kBytes = kBars + 2 * rows_stages<DP>() * 8;
 };
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   constexpr int kHalves = DP / 64, kHalfBytes = kRowsKeys * 128;  // a tile: [column half][key][128 bytes], swizzled
   const AttnParams& p = rp.a;
   float* stat = reinterpret_cast<float*>(smem + L::kStat);
+  float2* prev = reinterpret_cast<float2*>(smem + L::kPrev);
   int* fix = reinterpret_cast<int*>(smem + L::kFix);
   int* fixed = fix + kFixInts;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
@@ -246,11 +248,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   uint32_t qf[DP / 16][4];
   float o[DP / 8][4];
   float m[2], l[2];
-  // the stretches of kSumKeys keys before the one in o, against their own maxima: volatile keeps them out of the registers
-  volatile float carry[DP / 2];
-  float carry_m[2];
-  int stretch = 0;  // units in o
-  bool carried = false;
+  constexpr int kStretch = kSumKeys / kWarpKeys;  // units that a warp sums at a time
   int seen[2], common = 0, rows = 0, q0 = 0, len_q = 0;
   bool fresh = true, dead = false;
   int part_first = at.tile;  // first tile of the current (sequence, head) that this run takes
@@ -284,9 +282,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-      part_first = at.tile;
-      fresh = carried = false;
-      stretch = 0;
+      fresh = false;
     }
     // after a wait that gave up, the warp goes on without waiting (the status tells): the barriers between the
     // warps still see all of them
@@ -401,26 +397,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     }
 
 
-    const bool end = at.tile + 1 == at.tiles || u + 1 == count;
-    if (++stretch == kSumKeys / kWarpKeys || (end && carried)) {
-      float f[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        f[e] = carried ? moved(carry_m[e], m[e], sl2) : 0.f;
-        carry_m[e] = m[e];
-      }
-#pragma unroll
-      for (int i = 0; i < DP / 2; ++i) {
-        const float sum = carried ? fmaf(carry[i], f[(i >> 1) & 1], o[i / 4][i % 4]) : o[i / 4][i % 4];
-        if (!end) carry[i] = sum;
-        o[i / 4][i % 4] = end ? sum : 0.f;
-      }
-      carried = true;
-      stretch = 0;
-    }
-
-    // ---- the end of a (sequence, head), or of the run: join the key warps, write
-    if (end) {
+    // ---- the end of a (sequence, head), of the run or of a stretch: join the key warps, write
+    if (at.tile + 1 == at.tiles || u + 1 == count || (at.tile + 1 - part_first) % kStretch == 0) {
       const bool whole = part_first == 0 && at.tile + 1 == at.tiles;
       const int slot = 2 * blockIdx.x + (part_first == 0 ? 1 : 0);
 #pragma unroll
@@ -434,6 +412,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       }
       named_bar_sync(1, kRowsCompute);  // no warp reads the stage's K and V any more: it holds the accumulators now
       const bool patch = *fixed != 0;
+      // A stretch that is not the end goes to the workspace as a part does, its maxima and normalisers to one half of
+      // `prev`; the next one is added to it there, from that half to the other.  (As sums that the warps keep beside o this
+      // made 20 rows 17 % and 64 rows 29 % slower.)
+      const int ends = (at.tile - part_first) / kStretch;  // of stretches before
+      const bool more = at.tile + 1 < at.tiles && u + 1 < count;
       // [warp][row][DP] floats, columns swizzled by the row so that a warp's stores spread over the banks
       float* join = reinterpret_cast<float*>(stage);
 #pragma unroll
@@ -467,24 +450,37 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
           y[0] += a.x, y[1] += a.y, y[2] += a.z, y[3] += a.w, y[4] += b.x, y[5] += b.y, y[6] += b.z, y[7] += b.w;
         }
         const int token = r / p.group, qh = at.head * p.group + r % p.group;
-        const float inv = !whole ? 1.f : (norm == 0.f ? 0.f : 1.f / norm);
-        const int sees = patch ? keys_seen(token, len_q, at.len_k, p.causal) : 0;
+        const int64_t part = static_cast<int64_t>(slot) * rp.rows + r;
+        if (patch) {
+          const int sees = keys_seen(token, len_q, at.len_k, p.causal);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          y[e] *= inv;
-          if (patch) y[e] = put_back(y[e], fix, c + e, sees);
+          for (int e = 0; e < 8; ++e) y[e] = put_back(y[e], fix, c + e, sees);
         }
+        if (ends) {  // this thread's own sums of the stretches before
+          const float2 st = prev[((ends - 1) & 1) * 64 + r];
+          const float top = fmaxf(all, st.x), f0 = moved(st.x, top, sl2), f1 = moved(all, top, sl2);
+          const float* sum = rp.parts + part * p.head_dim + c;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fmaf(sum[e], f0, y[e] * f1);
+          norm = fmaf(st.y, f0, norm * f1);
+          all = top;
+        }
+        const float inv = !whole ? 1.f : (norm == 0.f ? 0.f : 1.f / norm);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] *= inv;
         if (whole) {
           *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (q0 + token) * p.o_ts + qh * p.o_hs + c) =
               make_uint4(pack_out<T>(y[0], y[1]), pack_out<T>(y[2], y[3]), pack_out<T>(y[4], y[5]), pack_out<T>(y[6], y[7]));
           if (c == 0 && p.lse)
             p.lse[static_cast<int64_t>(q0 + token) * p.q_heads + qh] = norm == 0.f ? -INFINITY : fmaf(all, p.scale, logf(norm * kProbUnit<T>));
         } else {
-          const int64_t part = static_cast<int64_t>(slot) * rp.rows + r;
           float4* dst = reinterpret_cast<float4*>(rp.parts + part * p.head_dim + c);
           dst[0] = make_float4(y[0], y[1], y[2], y[3]);
           dst[1] = make_float4(y[4], y[5], y[6], y[7]);
-          if (c == 0) *reinterpret_cast<float2*>(rp.stats + part * 2) = make_float2(all, norm);
+          if (c == 0) {
+            if (more) prev[(ends & 1) * 64 + r] = make_float2(all, norm);
+            else *reinterpret_cast<float2*>(rp.stats + part * 2) = make_float2(all, norm);
+          }
         }
       }
       if (patch) {
@@ -492,6 +488,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         for (int i = tid; i < kFixInts; i += kRowsCompute) fix[i] = INT_MAX;
         if (tid == 0) *fixed = 0;
       }
+      if (!more) part_first = 0;  // of the next (sequence, head), if this run takes one
       fence_proxy_async_smem();      // these accesses before the stage's next TMA write
       named_bar_sync(1, kRowsCompute);  // and before the next statistics
       fresh = true;

@@ -555,3 +555,21 @@ def test_outputs_in_place_of_the_queries(new):
     here = q.clone()
     ops.attention_paged(here, kc, vc, table, cu, ints(lens), new, out=here)
     assert torch.equal(here, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group", [1, 4, 16, 32])
+def test_few_rows_over_several_stretches(group, dtype):
+    """Contexts longer than what a warp sums at a time, each inside one block's share: values and infinities of all stretches."""
+    g = generator(29)
+    n, d, seqs = 140001, 64, 300
+    k, v = (rand(g, n, 1, d, dtype=dtype) for _ in range(2))
+    v[70000, 0, 7], v[-1, 0, 5], v[-1, 0, 7] = -math.inf, math.inf, math.inf  # the last key: the second row's alone
+    kc, vc, table = paged_of(k, v, 1024)
+    q = rand(g, 2 * seqs, group, d, dtype=dtype)
+    out, lse = ops.attention_paged(q, kc, vc, table.expand(seqs, -1).contiguous(), ints([2 * i for i in range(seqs + 1)]),
+                                   ints([n] * seqs), 2, return_lse=True)
+    assert ops.attention_status() == 0
+    for s in (0, 148, seqs - 1):
+        at = slice(2 * s, 2 * s + 2)
+        oracle.check(out[at], lse[at], *oracle.attend(q[at], k, v, 0.125, True), f"sequence {s}")
