@@ -694,11 +694,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // it), out of the way of the registers: a row of more than kSumKeys keys needs it once a stretch.
       float carry[DP], carry_m = -INFINITY;
       bool carried = false;
-      if (n) ok = __all_sync(~0u, wait_long(s_full + s, done));
-      for (int j = 0; ok && j < n;) {
+      int seen_beat = -1;
+      for (int j = 0; j < n;) {
         const int start = j, stop = min(n, j + kTcStretch);
         for (; j < stop; ++j, ++done) {
-          ok = __all_sync(~0u, wait(s_full + s, done));
+          ok = __all_sync(~0u, mbar_wait_bounded(s_full + s, done & 1, p.status, j ? kAttnTimeout : 0u));
           if (!ok) break;
           tc_fence_after();
           uint32_t x[128];
@@ -780,6 +780,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(p_full + s);
+        }
+        if (!ok && j == 0) {
+          // The first scores, which may be an item away: as mbar_wait_beat, but out of the loop above (in it, or as a wait of
+          // its own before it, 2 to 3 % slower at head size 64).
+          const int now = __shfl_sync(~0u, *beat, 0);
+          ok = now != seen_beat;
+          seen_beat = now;
+          if (ok) continue;
+          atomicOr(p.status, kAttnTimeout);
         }
         if (!ok || j == n) break;
         ok = __all_sync(~0u, wait(o_done + s, done - 1));  // the next tile's product starts O anew

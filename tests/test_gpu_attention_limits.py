@@ -573,3 +573,22 @@ def test_few_rows_over_several_stretches(group, dtype):
     for s in (0, 148, seqs - 1):
         at = slice(2 * s, 2 * s + 2)
         oracle.check(out[at], lse[at], *oracle.attend(q[at], k, v, 0.125, True), f"sequence {s}")
+
+
+def test_items_behind_one_of_a_hundred_million_keys():
+    """The long item has one row, so that half of its block's softmax warps have nothing to do in it and wait for the next item's
+    first scores as long as it lasts."""
+    g = generator(30)
+    n, d, short, rows = 2 ** 27 - 4096, 8, 320, 200
+    k_lens, q_lens = [n] + [rows] * short, [1] + [rows] * short
+    q = torch.zeros(1 + rows * short, 1, d, dtype=F16, device="cuda")
+    k, v = (torch.zeros(n + rows * short, 1, d, dtype=F16, device="cuda") for _ in range(2))
+    v[:n, :, 0] = 1
+    for x, a in ((q, 1), (k, n), (v, n)):
+        x[a:] = rand(g, rows * short, 1, d, dtype=F16)
+    out, lse = ops.attention_packed(q, k, v, ints(oracle.sums(q_lens)), ints(oracle.sums(k_lens)), causal=False, return_lse=True)
+    assert ops.attention_status() == 0
+    assert out[0, 0].tolist() == [1.0] + [0.0] * 7 and abs(float(lse[0, 0]) - math.log(n)) <= 2.0 ** -19
+    for i in (0, 146, 147, 148, 293, 294, 295, 319):  # of the first block's second item and around
+        at, kat = slice(1 + rows * i, 1 + rows * (i + 1)), slice(n + rows * i, n + rows * (i + 1))
+        oracle.check(out[at], lse[at], *oracle.attend_block(q[at], k[kat], v[kat], d ** -0.5, False), f"sequence {i}")
