@@ -592,3 +592,83 @@ def test_items_behind_one_of_a_hundred_million_keys():
     for i in (0, 146, 147, 148, 293, 294, 295, 319):  # of the first block's second item and around
         at, kat = slice(1 + rows * i, 1 + rows * (i + 1)), slice(n + rows * i, n + rows * (i + 1))
         oracle.check(out[at], lse[at], *oracle.attend_block(q[at], k[kat], v[kat], d ** -0.5, False), f"sequence {i}")
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_most_sequences_and_many_heads(new):
+    """65535 sequences in one call (the few-rows kernel, and the tensor-core one as if each could bring 70 rows), and 4096 heads."""
+    g = generator(31)
+    n, d, page = 65535, 8, 8
+    q = rand(g, n, 1, d, dtype=F16)
+    kc, vc = (rand(g, 50, page, 1, d, dtype=F16) for _ in range(2))
+    table = torch.randint(0, 50, (n, 1), generator=g, device="cuda").int()
+    lens = torch.randint(0, page + 1, (n,), generator=g, device="cuda").int()
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    out, lse = ops.attention_paged(q, kc, vc, table, cu, lens, new, scale=0.5, return_lse=True)
+    k, v = (c[table[:, 0].long(), :, 0].double() for c in (kc, vc))
+    s = 0.5 * (q.double() @ k.transpose(1, 2))[:, 0]
+    s = s.masked_fill(torch.arange(page, device="cuda")[None] >= lens[:, None], -math.inf)
+    top = torch.logsumexp(s, 1)
+    p = torch.exp(s - torch.where(lens > 0, top, 0.0)[:, None])
+    want, size = (p[:, None] @ v)[:, 0], (p[:, None] @ v.abs())[:, 0]
+    # as the oracle's bound: scores are sums of 8 products, off by 10 * 2^-23 of theirs at most
+    e_s = (10 * 2.0 ** -23 * 0.5 * (q.double().abs() @ k.abs().transpose(1, 2))[:, 0]).amax(1, keepdim=True)
+    u = oracle.half_step(F16)
+    tol = size * (u + 2 * e_s + 2.0 ** -16 + 2.0 ** -19) + u * want.abs() + 2.0 ** -25
+    assert bool(((out[:, 0].double() - want).abs() <= tol).all())
+    empty = lens == 0
+    assert bool((lse[empty] == -math.inf).all()) and bool(((lse[:, 0] - top).abs()[~empty] <= 2.0 ** -16).all())
+    h = 4096
+    q, k, v = (rand(g, 5, h, d, dtype=BF16) for _ in range(3))
+    want = oracle.attend_block(q, k, v, 0.3, True)
+    for name, out, lse, rows in every_way(q, k, v, 0.3, True, (1, 5)):
+        oracle.check(out, lse, *[w[rows] for w in want], name)
+
+
+def test_offsets_of_queries_and_outputs_beyond_32_bits():
+    """Heads and tokens of q, k, v and out far apart in one wide buffer."""
+    if torch.cuda.mem_get_info()[0] < 30 * 2 ** 30:
+        pytest.skip("needs 30 GB")
+    g = generator(32)
+    flat = torch.empty(10 * 2 ** 30, dtype=BF16, device="cuda")
+    hq, d, n = 2, 64, 3
+    far = (2 ** 32 + 2 ** 20) // 8 * 8
+    def wide(start, heads, across):  # [n, heads, d] with heads (or tokens) 2^32 elements apart
+        strides = (d, far, 1) if across == "heads" else (far // 2, d, 1)
+        t = torch.as_strided(flat, (n, heads, d), strides, start)
+        t.copy_(rand(g, n, heads, d, dtype=BF16))
+        return t
+    for across in ("heads", "tokens"):
+        q, k, v, out = (wide(4096 * i, hq, across) for i in range(4))
+        want = oracle.attend_block(q.contiguous(), k.contiguous(), v.contiguous(), 0.125, True)
+        cu = ints([0, n])
+        ops.attention_packed(q, k, v, cu, cu, out=out)
+        oracle.check(out.contiguous(), None, *want, across)
+        kc, vc, table = paged_of(k.contiguous(), v.contiguous())
+        for rows in (n, 1):
+            out.zero_()
+            ops.attention_paged(q[n - rows:], kc, vc, table, ints([0, rows]), cu[1:], 40 if rows == n else 1, out=out[n - rows:])
+            oracle.check(out[n - rows:].contiguous(), None, *[w[n - rows:] for w in want], across)
+    assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("n,rows", [(4, 2560), (20, 2560), (128, 2560), (60, 700)])
+def test_offsets_that_go_back_stay_inside_the_workspace(n, rows):
+    """Every second sequence has all query rows again: far more work than rows and sequences suggest.  Only the workspace's own
+    bytes are written."""
+    import random
+
+    rng, g = random.Random(n), generator(33)
+    q = rand(g, rows, 2, 64, dtype=F16)
+    kc, vc = (rand(g, 40, 16, 1, 64, dtype=F16) for _ in range(2))
+    lens = [rng.choice([100, 640, 9000, 30000]) for _ in range(n)]
+    table = torch.randint(0, 40, (n, 1875), generator=g, device="cuda").int()
+    size = ops.attention_paged_workspace(q, kc, n, rows).numel()
+    assert size
+    buffer = torch.full((size + 2 ** 24,), 0x5a, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 1000.0)
+    ops.attention_paged(q, kc, vc, table, ints([i % 2 * rows for i in range(n + 1)]), ints(lens), rows, out=out,
+                        workspace=buffer[:size])
+    assert ops.attention_status() == 0
+    assert bool((buffer[size:] == 0x5a).all())
+    assert bool((out.abs() < 100).all())  # rows of several sequences hold one of theirs
