@@ -203,7 +203,12 @@ bool kv_maps(const AexrtB200AttentionDesc* d, const AttnParams& p, bool paged, u
   return true;
 }
 
-// Query rows per sequence and kv head that the few-rows kernel takes; 0: the tensor-core kernel's.
+// Query rows per sequence and kv head that the few-rows kernel takes; 0: the tensor-core kernel's.  The few-rows kernel
+// against the tensor-core one, in us (8 kv heads of 128, bf16): 64 contexts of 4096 keys 181 against 287 with 20 rows, 187
+// against 287 with 32, 305-326 against 291 with 36 and 314-345 against 292 with 64; 16 of 4096 65 against 90 with 32, 97 and
+// 105 against 90 with 36 and 64; 4 of 8192 50 against 91 with 32, 69 and 80 against 91 with 36 and 64; one of 30000 69
+// against 84 with 32, 91 and 114 against 84 with 36 and 64.  So up to 32 rows it is the faster one everywhere, and from 33
+// to 64 over 4 contexts; over one, 16 or 64 a border of 32 would be faster.
 uint32_t few_rows(const AexrtB200AttentionDesc* d) {
   const uint64_t rows = static_cast<uint64_t>(d->max_q) * (d->q_heads / d->kv_heads);
   return rows <= 64 ? static_cast<uint32_t>(rows) : 0;
@@ -273,8 +278,10 @@ uint64_t tc_items(const AexrtB200AttentionDesc* d) {
   return each * d->kv_heads;
 }
 
-// Whether a paged call's items are split over their keys: when there are at most 3 for every 2 SMs (beyond that they even
-// out by themselves; two requests of 1024 tokens, 272 items, gain nothing) and a table row can hold keys for two parts.
+// Whether a paged call's items are split over their keys: when there are at most 3 for every 2 SMs and a table row can hold
+// keys for two parts.  Beyond, items even out by themselves, whole against split in us (32 heads over 8 of 128): two requests
+// of 1024 tokens (256 items) over 16384 keys 565 against 568, over 32768 1217 against 1225; one of 2048 over 16384 572
+// against 586.  Below, 64 tokens over 30000 keys take 391 whole and 66-69 split.
 // Without the table's columns (the workspace's size is asked for before there is a table) as for a long row.
 bool tc_splits(const AexrtB200AttentionDesc* d) {
   const uint64_t keys = static_cast<uint64_t>(d->table_columns) * d->page_size;

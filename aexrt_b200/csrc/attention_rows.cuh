@@ -12,8 +12,8 @@
 // running maximum and the accumulators of its keys, joined once per (sequence, head) through shared
 // memory.  A fifth warp loads, one TMA box per page, ahead across the sequences' borders: with the
 // loads and their page lookups in the computing warps (cp.async), those spent 945 instructions a unit and
-// the kernel reached 3.1 TB/s at 64 x 4096 keys, 8 heads of 128; now 185 us, 5.8 TB/s, which is what the
-// loads alone reach.  With 33 to 64 rows the warps' products bound it, at 3.0 to 3.3 TB/s.
+// the kernel reached 3.1 TB/s at 64 x 4096 keys, 8 heads of 128; now 174 to 181 us, 5.9 to 6.2 TB/s, which is what the
+// loads alone reach.  With 33 to 64 rows the warps' products bound it, at 3.1 to 3.5 TB/s.
 #pragma once
 #include <climits>
 

@@ -34,10 +34,14 @@
 // holds a whole row of S) and 72 for the others, 2 * 216 + 72 = 3 * 168 as launched.
 // TMEM columns: S 0-127, P0 128-191, P1 192-255, O0 256-, O1 384-.
 //
-// Measured (32 heads over 8, head size 128, bf16, 1000 W limit): one prompt of 16384 tokens 1.69 ms (1305 TFLOP/s) at
-// first, 1.90 ms in long runs at 1.55 GHz; 19 ragged prompts of 15001 tokens 211 us; 2 x 1024 tokens over 32768 cached keys
-// 473 us.  In long prompts the tensor pipe is 64 % active; ragged ones lose 9000 clocks an item to the last product's
-// latency and the output, which warps of their own did not win back (registers: 176 / 80 / 80; 260 -> 285 us).
+// Rows of more than 16384 keys are summed in stretches (kSumKeys): O starts anew and the sums before go to fp32 ones in
+// local memory, since the registers hold a row of S.
+//
+// Measured (32 heads over 8, head size 128, bf16, 1000 W limit; boxes and the length of the run differ): one prompt of
+// 16384 tokens 1.69 ms (1305 TFLOP/s) in the first second, 1.95 to 1.97 ms in long runs at 1.55 GHz; 19 ragged prompts of
+// 15001 tokens 213 to 226 us; 2 x 1024 tokens over 32768 cached keys 475 to 560 us.  In chunks and long prompts the
+// tensor pipe is 64 % active; ragged ones lose 9000 clocks an item to the last product's latency and the output, which
+// warps of their own did not win back (registers: 176 / 80 / 80; 260 -> 285 us).
 #pragma once
 #include <climits>
 
@@ -135,7 +139,10 @@ struct TcSplit {
 };
 
 // Numbers the items of a call: descending in key tiles while a warp can hold every sequence's lengths
-// (kHeld per lane), else by sequence.  Asked for ascending numbers, by a whole warp.
+// (kHeld per lane), else by sequence.  Asked for ascending numbers, by a whole warp.  By length against by sequence, in
+// us (32 heads over 8 of 128, causal): 19 ragged prompts of 15001 tokens 210-231 against 271-274, 8 of 13870 425-459
+// against 439-449, 100 of 42775 490-520 against 492-501; but 40 short ones of 3867 tokens 50 against 47 and 32 of 512
+// 153-168 against 140-153, where each search costs more than the order saves.
 template <bool kPaged>
 struct TcFinder {
   static constexpr int kHeld = 4;

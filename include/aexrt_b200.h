@@ -459,11 +459,13 @@ int aexrt_b200_act_quantize_f16_noalloc(const void* x, uint32_t n, uint32_t c, u
  *
  *   - Lengths live on the device, so a captured graph replays with other lengths.  Offsets and
  *     lengths are cut to the tensors' extents: nothing outside them is read or written.  Rows of
- *     q behind the last sequence are not read, and their rows of out and lse are left as they were.
+ *     q behind the last sequence do not matter, and their rows of out and lse are left as they were.
  *   - Nothing that a row does not see reaches its output, NaN and infinities in masked places,
  *     in unused cache rows and in neighbouring sequences included.  Infinite and NaN values that a
- *     row sees make its outputs infinite or NaN (an infinity whose probability rounds to 0 gives NaN); a NaN
- *     or +inf score makes its row NaN.
+ *     row sees make its outputs infinite or NaN (an infinity whose probability rounds to 0 gives NaN or stays); a NaN
+ *     or +inf score makes its row and its lse NaN; a row whose scores are all -inf is one that sees no key.
+ *   - Sums of 16384 keys at a time are taken on the tensor cores, which cut each term to 2^-25 of the sum, and
+ *     joined in fp32.  Finite values give finite outputs as long as len_k * 2^8 * |v| is in fp32's range.
  *   - head_dim: a multiple of 8 from 8 to 128; q_heads / kv_heads: at most 128.  Pointers 16-byte
  *     aligned, strides (elements) multiples of 8 (that of a dimension of size 1 is ignored), each
  *     head's head_dim elements contiguous.
@@ -512,8 +514,9 @@ int aexrt_b200_attention_paged(const AexrtB200AttentionDesc* desc, const void* q
 uint64_t aexrt_b200_attention_paged_workspace(const AexrtB200AttentionDesc* desc);
 
 /* Status of the current device's attention kernels since the last read: waits for all work on the
- * device, on every stream, then reads and clears it in one step (so not while a stream is captured).  BAD_PAGE: a block table entry outside the cache was met.  TIMEOUT: a wait inside
- * a kernel gave up, and outputs of that call are incomplete. */
+ * device, on every stream, then reads and clears it in one step (so not while a stream is captured).
+ * BAD_PAGE: a block table entry outside the cache was met.  TIMEOUT: a wait inside a kernel gave
+ * up, and outputs of that call are incomplete. */
 #define AEXRT_B200_ATTENTION_BAD_PAGE 1u
 #define AEXRT_B200_ATTENTION_TIMEOUT 2u
 int aexrt_b200_attention_status(uint32_t* status);
@@ -542,7 +545,8 @@ int aexrt_b200_page_tables(const int32_t* ctx_lens, const int32_t* new_lens, uin
 
 /* Writes rows k[t], v[t] ([kv_heads][head_dim] of 16-bit elements) to slot slot_map[t] of the
  * caches; slots below 0 or at and above num_pages * page_size (below 2^31) are skipped.  Two tokens
- * with the same slot leave each 16-byte piece from one of them.  The caches overlap neither k, v nor each other.  Strides as in AexrtB200AttentionDesc. */
+ * with the same slot leave each 16-byte piece from one of them.  The caches overlap neither k, v nor
+ * each other.  Strides as in AexrtB200AttentionDesc. */
 int aexrt_b200_kv_append(const void* k, const void* v, uint32_t tokens, uint32_t kv_heads, uint32_t head_dim,
                          uint64_t k_token_stride, uint64_t k_head_stride, uint64_t v_token_stride,
                          uint64_t v_head_stride, const int32_t* slot_map, void* k_cache, void* v_cache,
