@@ -1,8 +1,10 @@
 """Arguments of the token-sequence wrappers that no call can take: refused with a ValueError before anything is launched (no GPU)."""
+import ctypes
+
 import pytest
 import torch
 
-from aexrt_b200 import ops
+from aexrt_b200 import _native, ops
 
 H, I = torch.float16, torch.int32
 
@@ -64,3 +66,18 @@ def test_append_of_more_rows_than_32_bits_count():
     cache = torch.zeros(2, 16, 2, 64, dtype=H)
     with pytest.raises(ValueError, match="out of range"):
         ops.kv_append(k, k, torch.zeros(4, dtype=I), cache, cache)
+
+
+@pytest.mark.parametrize("scale,taken", [(1.01e38, False), (3.4e38, False), (1e38, True), (0.0, True), (1.401298464e-45, True)])
+def test_scales_from_0_to_1e38(scale, taken):
+    """Through the C entry points, on a description of no rows, which is taken without a launch."""
+    d = _native.AexrtB200AttentionDesc(struct_size=ctypes.sizeof(_native.AexrtB200AttentionDesc), dtype=0, num_seqs=1, q_tokens=0,
+                                       max_q=1, q_heads=2, kv_heads=1, head_dim=64, causal=1, scale=scale, kv_tokens=4, page_size=16,
+                                       table_columns=1, table_stride=1, q_token_stride=128, q_head_stride=64, out_token_stride=128,
+                                       out_head_stride=64, k_token_stride=64, k_head_stride=64, k_page_stride=1024,
+                                       v_token_stride=64, v_head_stride=64, v_page_stride=1024)
+    lib, at = _native.load(), ctypes.byref(d)
+    for got in (lib.aexrt_b200_attention_packed(at, *[None] * 8), lib.aexrt_b200_attention_paged(at, *[None] * 9, 0, None)):
+        assert got == int(taken)
+        assert taken or "scale must be from 0 to 1e38" in _native.last_error()
+    assert lib.aexrt_b200_attention_paged_workspace(at) == (0 if taken else 2 ** 64 - 1)
